@@ -1,11 +1,12 @@
 // Implicit-GEMM convolution (K1 forward / K2 data gradient) with prefetch depth 2: one wave per SIMD,
 // a 128 x 128 (or 128 x 64) output sub-tile per wave, two LDS buffers and two tiles of loads in flight.
 //
-// Why (profiles/r9a_gemmref_hipblaslt_vs_ours_b1024.txt): on the compute-bound ResNet-50 GEMMs the
-// 256 x 256 tile of conv_gemm_glds_kernel - 8 waves of 128 x 64, a 2-buffer ring waited to vmcnt(0) every
-// k-step, so ONE tile is in flight while one is computed - runs 945-1190 TF where the library's
-// hand-written 256 x 256 kernel runs 1313-1619 TF.  That kernel's structure (read from its code object:
-// 4 waves, 256 accumulator registers per lane, 130 KB of LDS) is what this file builds in HIP:
+// Why: on the compute-bound ResNet-50 GEMMs the 256 x 256 tile of conv_gemm_glds_kernel - 8 waves of 128 x 64, a
+// 2-buffer ring waited to vmcnt(0) every k-step, so ONE tile is in flight while one is computed - runs 945-1190 TF
+// where plain library GEMMs of the same sizes run 1313-1619 TF.  The layout follows from the LDS port: a wave's
+// (WTM + WTN) x 32 fragment reads feed WTM x WTN / 256 MFMAs, so 128 x 128 a wave reads a third less per MFMA than
+// 128 x 64; its accumulators are 128 * 128 / 64 = 256 registers a lane, which one wave per SIMD has to spare, and two
+// stages of (256 + 256) rows x 128 B are 128 KB of the 160 KB of LDS:
 //
 //  * 4 waves in 2 x 2, each a (TM/2) x (BN/2) sub-tile: a 128 x 128 sub-tile issues one ds_read_b128 per
 //    4 MFMAs (the 8-wave 128 x 64 sub-tile: one per 2.7), so the LDS read port stays far from saturation;
@@ -146,8 +147,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void conv_deep_kernel(const ConvPa
   const __amdgpu_buffer_rsrc_t rsZ = make_rsrc(p.A, 0);
   // The per-lane source offsets change only at a tap boundary (per-row validity and the tap's pixel shift);
   // the channel slice of a k-step is a wave-uniform byte offset passed as the load's SGPR offset, so a
-  // k-step inside a tap costs no VALU at all (the library GEMM's loop has ~7 VALU per k-step; a per-piece
-  // address recompute cost this kernel ~30 points of MFMA busy: profiles/r9d_*).
+  // k-step inside a tap costs no VALU at all (a per-piece address recompute cost this kernel ~30 points of
+  // MFMA busy).
   int u_tap = 0, u_ci = 0;
   int u_pk = s_tap[0];
   unsigned a_vb[AL];
