@@ -29,7 +29,11 @@ OUT = os.path.join(PKG, "_C.so")
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
+# no packed fp32 arithmetic (v_pk_{add,mul,fma}_f32): some of its operand forms have given wrong results on
+# MI355X now and then, and -O3 forms them from ordinary float code (hipcc's host pass warns that it does not know
+# the feature: harmless)
 KERNEL_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-fp-atomics",
+                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                 "-Wno-unused-result", "-D__HIP_PLATFORM_AMD__=1"]
 
 
