@@ -1082,6 +1082,7 @@ class PeerComm {
 }  // namespace
 
 void register_loader(pybind11::module& m);  // loader.cpp: native image-folder loader
+void register_block_ops(pybind11::module& m);  // block_bindings.cpp: dropout / RMS norm / 8-bit linear block
 void bn_set_reduce_blocks(int n, int chb);
 void bn_set_unroll(int v);
 bool bn_res_coef_ok(bool mask);
@@ -1210,6 +1211,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("normalize_u8", &normalize_u8);
   m.def("input_u8", &input_u8);
   register_loader(m);
+  register_block_ops(m);
   m.def("bn_set_reduce_blocks", &bn_set_reduce_blocks, pybind11::arg("n"), pybind11::arg("chb") = 0);
   m.def("bn_act_maxpool", &bn_act_maxpool);
   m.def("bn_set_unroll", [](bool v) { bn_set_unroll(v ? 1 : 0); });

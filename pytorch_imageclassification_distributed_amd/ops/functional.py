@@ -24,6 +24,9 @@ import os
 import torch
 import torch.nn.functional as F
 
+from .fp8_blocks import (FLOATS, Fp8Blocks, dequantize_ref, drop_ref, drop_threshold, linear_fp8_ref, quantize_rows_ref,
+                         quantize_tiles_ref, rms_norm_fp8_ref, rms_norm_ref)
+
 _BACKEND = os.environ.get("IMGCLS_BACKEND", "auto")  # auto | hip | torch
 
 
@@ -213,6 +216,182 @@ def dropout(x, p, training):
     if use_hip(x):
         return _hip().dropout(x, p)
     return F.dropout(x, p, True)
+
+
+# ---------------------------------------------------------------------------
+# pre-norm 8-bit linear block: counter-based dropout, root-mean-square norm, 8-bit products
+# ---------------------------------------------------------------------------
+def _check_floats(name, x):
+    if x.dtype not in FLOATS:
+        raise TypeError(f"{name}: x is {x.dtype}, expected bfloat16, float16 or float32")
+
+
+def _check_like(name, what, t, x):
+    if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+        raise ValueError(f"{name}: {what} must match x ({x.dtype} {tuple(x.shape)} on {x.device}), "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_drop(name, x, p, seed, offset):
+    """The drop threshold of ``p``; refuses seeds the kernels cannot take."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"{name}: p must be in [0, 1], got {p}")
+    if torch.is_tensor(seed):
+        if seed.dtype != torch.int64 or tuple(seed.shape) != (2,) or seed.device != x.device or not seed.is_contiguous():
+            raise ValueError(f"{name}: a seed tensor is int64 [seed, offset] on {x.device}")
+        if offset != 0:
+            raise ValueError(f"{name}: a seed tensor holds the offset itself")
+    elif seed is None:
+        if offset != 0:
+            raise ValueError(f"{name}: offset without a seed")
+    elif not (0 <= int(seed) < 2**64 and 0 <= int(offset) < 2**64):
+        raise ValueError(f"{name}: seed and offset are 64-bit unsigned, got {seed}, {offset}")
+    return drop_threshold(p)
+
+
+def _seed_values(seed, offset):
+    """Host values for the reference path."""
+    if seed is None:
+        seed = torch.randint(0, 2**63 - 1, (2,), dtype=torch.int64)
+    if torch.is_tensor(seed):
+        seed, offset = (v % 2**64 for v in seed.tolist())
+    return int(seed), int(offset)
+
+
+def dropout_counter(x, p, training=True, seed=None, offset=0, residual=None):
+    """``[residual +] dropout(x, p)`` whose mask is a function of (element index, ``seed``, ``offset``) and is never
+    stored: the backward pass makes it again.  The sum is rounded once, to x's type.
+
+    ``seed``: a 64-bit integer; or an int64 tensor ``[seed, offset]`` on x's device, read when the kernels run (a captured
+    graph sees the values it holds at each replay; changing it between forward and backward is an error); or None, which
+    draws both from the device's generator.  Every (seed, offset) pair is an independent mask over up to 2^67 elements.
+    ``p`` is rounded to a multiple of 2^-16; the kept values are scaled by 1 / (1 - that).  Elements are numbered in
+    row-major order whatever the strides; the result is row-major.  A dropped infinity or NaN leaves 0.
+    """
+    _check_floats("dropout_counter", x)
+    _check_like("dropout_counter", "residual", residual, x)
+    t = _check_drop("dropout_counter", x, p, seed, offset)
+    if not training or t == 0:
+        if residual is None:
+            return x
+        return _hip().dropout_counter(x, residual, 0, 0, 0) if use_hip(x) else x + residual
+    if use_hip(x):
+        return _hip().dropout_counter(x, residual, t, seed, offset)
+    y = drop_ref(x.contiguous().float(), t, *_seed_values(seed, offset))
+    return (y if residual is None else y + residual.float()).to(x.dtype)
+
+
+def _norm_args(name, x, norm, residual):
+    _check_floats(name, x)
+    _check_like(name, "residual", residual, x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: x needs a last dimension of at least 1, got {tuple(x.shape)}")
+    w = norm.weight
+    if w is not None and (tuple(w.shape) != (x.shape[-1],) or w.device != x.device or w.dtype not in FLOATS):
+        raise ValueError(f"{name}: weight must be [{x.shape[-1]}] on {x.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    if w is None and tuple(norm.normalized_shape) != (x.shape[-1],):
+        raise ValueError(f"{name}: the norm is over {tuple(norm.normalized_shape)}, x's rows have {x.shape[-1]}")
+    if use_hip(x) and x.shape[-1] > _hip().C.rms_max_cols():
+        raise ValueError(f"{name}: rows of at most {_hip().C.rms_max_cols()} columns, got {x.shape[-1]}")
+    return w, norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
+
+
+def rms_norm(x, norm, residual=None, p=0.0, training=True, seed=None, offset=0):
+    """Root-mean-square norm over the last dimension (``norm``: an ``nn.RMSNorm``), with the residual's addition and the
+    dropout before it in the same pass: ``h = residual + dropout_counter(x, p)``, ``y = h / sqrt(mean(h^2) + eps) * weight``.
+
+    Returns ``y``, or ``(y, h)`` with a ``residual`` (``h``, rounded to x's type, is the next layer's residual and what
+    is normalised).  ``seed`` / ``offset`` as in ``dropout_counter``.  Sums and statistics are float32.
+    """
+    w, eps = _norm_args("rms_norm", x, norm, residual)
+    t = _check_drop("rms_norm", x, p, seed, offset) if training else 0
+    if use_hip(x):
+        return _hip().rms_norm(x, w, eps, residual, t, seed, offset)
+    return rms_norm_ref(x.contiguous(), w, eps, residual, t, *(_seed_values(seed, offset) if t else (0, 0)))
+
+
+def rms_norm_fp8(x, norm, residual=None):
+    """``rms_norm`` with an 8-bit result for ``matmul_fp8``: ``Fp8Blocks`` over the flattened rows (1 x 128 blocks,
+    quantised from the float32 values), or ``(Fp8Blocks, h)`` with a ``residual``.
+
+    For inference: it has no gradient and refuses inputs that ask for one (training: ``rms_norm``, then ``linear_fp8``)."""
+    w, eps = _norm_args("rms_norm_fp8", x, norm, residual)
+    _refuse_grad("rms_norm_fp8", x, residual, w)
+    if use_hip(x):
+        return _hip().rms_norm_fp8(x, w, eps, residual)
+    out, h = rms_norm_fp8_ref(x.contiguous(), w, eps, residual)
+    return out if residual is None else (out, h)
+
+
+def _refuse_grad(name, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train through linear_fp8")
+
+
+def quantize_fp8(x):
+    """Activations ``[..., K]`` -> ``Fp8Blocks`` over the flattened rows, one scale for each 1 x 128 block."""
+    _check_floats("quantize_fp8", x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"quantize_fp8: x needs a last dimension of at least 1, got {tuple(x.shape)}")
+    _refuse_grad("quantize_fp8", x)
+    x2 = x.reshape(-1, x.shape[-1])
+    return _hip().quantize_fp8(x2) if use_hip(x) else quantize_rows_ref(x2)
+
+
+def quantize_fp8_weight(w):
+    """A weight ``[N, K]`` -> ``Fp8Blocks`` with one scale for each 128 x 128 tile (laid out once, for serving)."""
+    _check_floats("quantize_fp8_weight", w)
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
+        raise ValueError(f"quantize_fp8_weight: a weight is [N, K], got {tuple(w.shape)}")
+    w = w.detach()
+    return _hip().quantize_fp8_weight(w) if use_hip(w) else quantize_tiles_ref(w)
+
+
+def matmul_fp8(a, b, bias=None, act=None, out_dtype=torch.bfloat16):
+    """``act(a @ b.T + bias)`` of 8-bit blocks: a ``[M, K]`` with 1 x 128 blocks, b ``[N, K]`` with 1 x 128 blocks or
+    128 x 128 tiles -> ``[M, N]`` in ``out_dtype``.  ``act``: None, 'relu' or 'silu'.
+
+    Accumulators are float32; the matrix instructions cut the products of a 128-block at about 2^-16 of the largest, so a
+    float32 result is within 2^-15 or so of the exact sum's norm.  For inference: no gradient (training: ``linear_fp8``)."""
+    if a.tile != 1:
+        raise ValueError("matmul_fp8: a needs 1 x 128 blocks (quantize_fp8, rms_norm_fp8)")
+    if a.shape[1] != b.shape[1]:
+        raise ValueError(f"matmul_fp8: inner sizes differ: {a.shape} and {b.shape}")
+    if a.device != b.device:
+        raise ValueError(f"matmul_fp8: a on {a.device}, b on {b.device}")
+    if bias is not None and (tuple(bias.shape) != (b.shape[0],) or bias.device != a.device or bias.dtype not in FLOATS):
+        raise ValueError(f"matmul_fp8: bias must be [{b.shape[0]}] on {a.device}")
+    if act not in (None, "relu", "silu"):
+        raise ValueError(f"matmul_fp8: act {act!r}")
+    if out_dtype not in FLOATS:
+        raise ValueError(f"matmul_fp8: out_dtype {out_dtype}")
+    _refuse_grad("matmul_fp8", bias)
+    if use_hip(a.q):
+        return _hip().matmul_fp8(a, b, bias, act, out_dtype)
+    y = dequantize_ref(a) @ dequantize_ref(b).t()
+    return _act(y if bias is None else y + bias.float(), act).to(out_dtype)
+
+
+def linear_fp8(x, lin, act=None):
+    """``linear`` with an 8-bit forward and data gradient (``lin``: an ``nn.Linear`` with float32, bfloat16 or float16
+    parameters; the weight is quantised at every call, so an optimiser may change it in between).
+
+    ``y = act(q(x) q(w)^T + b)`` in x's type, 1 x 128 blocks for x and dy, 128 x 128 for w; ``dx = q(dy) q(w)``;
+    ``dw = dy^T x`` on x and dy rounded to bfloat16 with float32 sums; ``db`` = float32 column sums.  ``act``: None or
+    'relu' (whose gradient is masked before dy is quantised)."""
+    _check_floats("linear_fp8", x)
+    w, b = lin.weight, lin.bias
+    if act not in (None, "relu"):
+        raise NotImplementedError(act)
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"linear_fp8: x {tuple(x.shape)} does not fit weight {tuple(w.shape)}")
+    if w.shape[0] < 1 or w.shape[1] < 1 or w.dtype not in FLOATS or (b is not None and b.dtype not in FLOATS):
+        raise ValueError(f"linear_fp8: weight {w.dtype} {tuple(w.shape)}")
+    if w.device != x.device or (b is not None and b.device != x.device):
+        raise ValueError(f"linear_fp8: x on {x.device}, weight on {w.device}")
+    x2 = x.reshape(-1, x.shape[-1])
+    y = _hip().linear_fp8(x2, w, b, act) if use_hip(x) else linear_fp8_ref(x2, w, b, act)
+    return y.view(*x.shape[:-1], w.shape[0])
 
 
 class ConcatPlan:

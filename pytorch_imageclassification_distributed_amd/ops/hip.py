@@ -19,10 +19,10 @@ from __future__ import annotations
 import sys
 import types
 
-from ._hip import adam, common, convbn, gemm, misc, pool, shadows, streams
+from ._hip import adam, block, common, convbn, gemm, misc, pool, shadows, streams
 
 _PARTS = {"common": common, "shadows": shadows, "gemm": gemm, "streams": streams, "pool": pool, "convbn": convbn,
-          "misc": misc, "adam": adam}
+          "misc": misc, "adam": adam, "block": block}
 # every public and private name of the parts, by owning module
 _OWNER = {}
 for _m in _PARTS.values():
