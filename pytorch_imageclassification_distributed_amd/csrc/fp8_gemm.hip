@@ -6,6 +6,8 @@
 // The instruction aligns its 128 products to the largest before it adds them: sums come out within 2^-16 of the exact
 // ones (1.5e-5 of the result's norm on normal data, whatever K; the bf16 instruction gives 9e-8), which a bf16 or fp16
 // output does not show.
+#include <type_traits>
+
 #include "conv_common.h"
 
 namespace {
@@ -20,18 +22,26 @@ struct Fp8Gemm {
   int ldsa, ldsb;    // scale bytes a scale row (multiples of 4)
   int bshift;        // log2 of the B rows that share a scale row: 0 or 7
   long ldc;
-  int act, ctype;    // ctype: 0 bf16, 1 fp16, 2 fp32
 };
 
+// output types (compile-time, as the activation is: a branch an element tripled the epilogue's code)
+enum { C_BF16 = 0, C_F16 = 1, C_F32 = 2 };
+
+template <int CT>
 DEVI void store_c(const Fp8Gemm& p, long i, float v) {
-  if (p.ctype == 0) ((bf16_t*)p.C)[i] = f2bf(v);
-  else if (p.ctype == 1) ((_Float16*)p.C)[i] = (_Float16)v;
+  if constexpr (CT == C_BF16) ((bf16_t*)p.C)[i] = f2bf(v);
+  else if constexpr (CT == C_F16) ((_Float16*)p.C)[i] = (_Float16)v;
   else ((float*)p.C)[i] = v;
+}
+template <int CT>
+DEVI uint32_t pack_c(float a, float b) {
+  if constexpr (CT == C_BF16) return pack2(a, b);
+  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
 // BM x BN tile on WM x WN waves, two LDS stages of one k-step each filled by LDS-DMA.  Rows past M or N read the last
 // row again (their results are not stored).
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int ACT, int CT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p) {
   constexpr int NW = WM * WN;
   constexpr int WTM = BM / WM, WTN = BN / WN, RM = WTM / 16, RN = WTN / 16;
@@ -142,14 +152,239 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int n = n0 + wn * WTN + j * 16 + fq * 4 + r;
-        if (n < p.N) store_c(p, (long)m * p.ldc + n, apply_act(acc[i][j][r] + (p.bias ? p.bias[n] : 0.f), p.act));
+        if (n < p.N) store_c<CT>(p, (long)m * p.ldc + n, apply_act(acc[i][j][r] + (p.bias ? p.bias[n] : 0.f), ACT));
       }
   }
 }
 
-template <int BM, int BN, int WM, int WN>
+// ---- the large tile ----
+// 256 x 256 on 4 waves of 128 x 128, one block a CU.  A k-step of a wave is 64 MFMAs fed by 32 ds_read_b128: (128 + 128)
+// rows x 128 B x 4 waves + the 64 KB that LDS-DMA writes are 192 KB a step through the LDS port, against 256 KB for
+// 8 waves of 128 x 64 (where the port, not the matrix pipe, would set the pace).  The 256 accumulators of a lane live in
+// AGPRs, the fragments of one k-step in 128 VGPRs; the step runs in two halves of four B fragments each (all eight A
+// fragments in both), so that every register is refilled where its last MFMA has been issued:
+//   first half of step kt (B 0-3):   B 4-7 of kt are read;
+//   middle: tile kt + 1 has landed, this buffer's reads have ended in every wave: the step's one barrier;
+//   second half (B 4-7):             the 16 LDS-DMA pieces of tile kt + 2 go into this buffer, and B 0-3 and, row by
+//                                    row, A of kt + 1 are read from the other one.
+// One memory instruction or two stand between two MFMAs; a tile has a whole step (64 x 32 cycles) to arrive.
+// The MFMAs are asm statements (accumulators pinned to AGPRs, order kept); each carries the two wait states between a
+// VALU write and a matrix read.
+template <int R>
+DEVI void mma_step(f32x4& acc, const i32x8& b, const i32x8& a, uint32_t sb, uint32_t sa) {
+  static_assert(R >= 0 && R < 4, "scale byte");
+  if constexpr (R == 0)
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+  else if constexpr (R == 1)
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+  else if constexpr (R == 2)
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+  else
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+}
+
+DEVI void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, int soff, char* lds_wave_base) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 16, voff, soff, 0, 0);
+}
+
+DEVI i32x8 frag8(const char* lo, const char* hi) {
+  const int4 l = *(const int4*)lo, h = *(const int4*)hi;
+  return (i32x8){l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
+}
+
+constexpr int BIG_STAGE = 512 * 128;
+constexpr int BIG_CST = 256 + 8;  // 16-bit elements a row of the staged output tile: 4 rows differ by 16 banks
+constexpr int BIG_BUF = 128 * BIG_CST * 2 > BIG_STAGE ? 128 * BIG_CST * 2 : BIG_STAGE;  // half of the output tile each
+
+template <int ACT, int CT>
+__global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
+  // two arrays, not one: hipcc makes an LDS read wait for every LDS-DMA that may write what it reads, and tells them
+  // apart by the array alone
+  __shared__ __attribute__((aligned(16))) char buf0[BIG_BUF];
+  __shared__ __attribute__((aligned(16))) char buf1[BIG_BUF];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid >> 1, wn = wid & 1;
+  const int gm = (p.M + 255) >> 8, gn = (p.N + 255) >> 8;
+  const int lin = xcd_remap(blockIdx.x, gm * gn);
+  // an XCD's consecutive tiles walk a band of 4 tile rows column by column: its L2 then holds 4 row panels and a few
+  // column panels at a time
+  const int band = lin / (4 * gn), first = band * 4, rows = min(gm - first, 4), rest = lin - band * 4 * gn;
+  const int m0 = __builtin_amdgcn_readfirstlane((first + rest % rows) * 256);
+  const int n0 = __builtin_amdgcn_readfirstlane((rest / rows) * 256);
+
+  // LDS-DMA sources: piece q of a wave is rows [64 wid + 8 q, + 8) of its 256; lane l brings 16-B chunk (l & 7) of row
+  // l >> 3, from source chunk (l & 7) ^ ((row >> 1) & 7), which takes two values over q.  Rows past the end are past
+  // the buffer resource: zeros.
+  const int lrow = lane >> 3, pch = lane & 7;
+  const long abytes = (long)(p.M - m0) * p.lda, bbytes = (long)(p.N - n0) * p.ldb;
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.A + (long)m0 * p.lda, abytes), rb = make_rsrc(p.B + (long)n0 * p.ldb, bbytes);
+  const __amdgpu_buffer_rsrc_t za = make_rsrc(p.A, 0);
+  const int lda = (int)p.lda, ldb = (int)p.ldb;
+  unsigned va[2], vb[2];
+#pragma unroll
+  for (int o = 0; o < 2; ++o) {
+    const int ch = (pch ^ ((lrow >> 1) + 4 * o)) * 16;
+    va[o] = (unsigned)((wid * 64 + lrow) * lda + ch);
+    vb[o] = (unsigned)((wid * 64 + lrow) * ldb + ch);
+  }
+  auto piece = [&](int kt, char* buf, int q, bool live) __attribute__((always_inline)) {
+    char* dst = buf + (wid * 64 + (q & 7) * 8) * 128;
+    if (q < 8) dma16(live ? ra : za, va[q & 1], kt * 128 + q * 8 * lda, dst);
+    else dma16(live ? rb : za, vb[q & 1], kt * 128 + (q - 8) * 8 * ldb, dst + 256 * 128);
+  };
+
+  const int fr = lane & 15, fq = lane >> 4;
+  // fragment i of a buffer: row 16 i + fr of the wave's 128, chunks fq and fq + 4 (the swizzle depends on fr alone)
+  const int oa = swz(wm * 128 + fr, fq), oah = swz(wm * 128 + fr, fq + 4);
+  const int ob = 256 * 128 + swz(wn * 128 + fr, fq), obh = 256 * 128 + swz(wn * 128 + fr, fq + 4);
+
+  // scales: a word holds four k-steps' bytes; a pair of steps takes bytes 0 and 1, then the words are shifted.  The next
+  // words are loaded four steps ahead.  An odd number of steps runs one more on zeros (the DMA pieces past the end come
+  // from an empty resource); its scale byte is cleared, so that padding cannot hold a NaN scale.
+  const int nk = p.nk;
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(p.As + (long)m0 * p.ldsa, (long)(p.M - m0) * p.ldsa);
+  const int vsa = (wm * 128 + fr) * p.ldsa;
+  const uint32_t* wsb = (const uint32_t*)(p.Bs + (long)(min(n0 + wn * 128, p.N - 1) >> 7) * p.ldsb);
+  const int words = (nk + 3) >> 2;
+  const uint32_t last = (nk & 3) ? (1u << (8 * (nk & 3))) - 1 : ~0u;
+  uint32_t sx[8], nx[8], sw, nw;
+  auto scales = [&](int word) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nx[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa, word * 4 + i * 16 * p.ldsa, 0);
+    nw = wsb[word];
+  };
+
+  f32x4 acc[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  asm volatile("s_nop 7");
+
+  i32x8 a[8], b[8];
+#pragma unroll
+  for (int q = 0; q < 16; ++q) piece(0, buf0, q, true);
+#pragma unroll
+  for (int q = 0; q < 16; ++q) piece(1, buf1, q, nk > 1);
+  scales(0);
+  wait_vmcnt<0>();
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] = frag8(buf0 + oa + i * 2048, buf0 + oah + i * 2048);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = frag8(buf0 + ob + j * 2048, buf0 + obh + j * 2048);
+
+  auto step = [&](auto rc, int kt) __attribute__((always_inline)) {
+    constexpr int P = decltype(rc)::value;  // kt & 1
+    auto cur = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf0; else return (char*)buf1; };
+    auto nxt = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf1; else return (char*)buf0; };
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+      const int i = t >> 2, j = t & 3;
+      mma_step<P>(acc[i][j], b[j], a[i], sw, sx[i]);
+      if ((t & 3) == 1 && t < 16) b[4 + (t >> 2)] = frag8(cur() + ob + (4 + (t >> 2)) * 2048, cur() + obh + (4 + (t >> 2)) * 2048);
+    }
+    wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    const bool live = kt + 2 < nk;
+#pragma unroll
+    for (int t = 0; t < 32; ++t) {
+      const int i = t >> 2, j = 4 + (t & 3);
+      mma_step<P>(acc[i][j], b[j], a[i], sw, sx[i]);
+      if (t < 16) piece(kt + 2, cur(), t, live);
+      if ((t & 3) == 2 && t < 16) b[t >> 2] = frag8(nxt() + ob + (t >> 2) * 2048, nxt() + obh + (t >> 2) * 2048);
+      if (j == 7) a[i] = frag8(nxt() + oa + i * 2048, nxt() + oah + i * 2048);
+    }
+  };
+  for (int kt = 0; kt < nk; kt += 2) {
+    if ((kt & 2) == 0) {
+      const uint32_t m = (kt >> 2) == words - 1 ? last : ~0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sx[i] = nx[i] & m;
+      sw = nw & m;
+      scales(min((kt >> 2) + 1, words - 1));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sx[i] >>= 16;
+      sw >>= 16;
+    }
+    step(std::integral_constant<int, 0>{}, kt);
+    step(std::integral_constant<int, 1>{}, kt + 1);
+  }
+  wait_vmcnt<0>();
+  // the last MFMAs' results before the first read of an accumulator: waits that every accumulator depends on
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]), "+a"(acc[i][4]), "+a"(acc[i][5]), "+a"(acc[i][6]), "+a"(acc[i][7]));
+  __syncthreads();
+  float bias[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = n0 + wn * 128 + j * 16 + fq * 4 + r;
+      bias[j][r] = p.bias != nullptr && n < p.N ? p.bias[n] : 0.f;
+    }
+  if constexpr (CT == C_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int m = m0 + wm * 128 + i * 16 + fr;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int n = n0 + wn * 128 + j * 16 + fq * 4 + r;
+          if (m < p.M && n < p.N) store_c<CT>(p, (long)m * p.ldc + n, apply_act(acc[i][j][r] + bias[j][r], ACT));
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
+  // 16-bit outputs go through LDS, so that rows leave in whole 16-B chunks of 512 contiguous bytes
+  uint16_t* ct = (uint16_t*)(wm == 0 ? buf0 : buf1);  // rows 0-127 and 128-255 of the tile
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = apply_act(acc[i][j][r] + bias[j][r], ACT);
+      *(uint2*)(ct + (i * 16 + fr) * BIG_CST + wn * 128 + j * 16 + fq * 4) = make_uint2(pack_c<CT>(v[0], v[1]), pack_c<CT>(v[2], v[3]));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __syncthreads();
+  uint16_t* C = (uint16_t*)p.C;
+  const int cc = (tid & 31) * 8;
+  const int nv = min(8, p.N - n0 - cc);
+  const bool vec = (p.ldc & 7) == 0;
+  for (int r = tid >> 5; r < 256 && m0 + r < p.M; r += 8) {
+    const uint4 v = *(const uint4*)((const uint16_t*)(r < 128 ? buf0 : buf1) + (r & 127) * BIG_CST + cc);
+    uint16_t* o = C + (long)(m0 + r) * p.ldc + n0 + cc;
+    if (vec && nv == 8) *(uint4*)o = v;
+    else {
+      const uint16_t* e = (const uint16_t*)&v;
+      for (int k = 0; k < nv; ++k) o[k] = e[k];
+    }
+  }
+}
+
+template <int ACT, int CT>
 void launch(const Fp8Gemm& p, hipStream_t s) {
-  hipLaunchKernelGGL((fp8_gemm_kernel<BM, BN, WM, WN>), dim3(cdiv(p.M, BM) * cdiv(p.N, BN)), dim3(64 * WM * WN), 0, s, p);
+  // (32-bit offsets inside a tile: 256 rows of at most 2^22 bytes)
+  if (p.bshift == 7 && p.M >= 512 && p.N >= 512 && p.lda <= (1 << 22) && p.ldb <= (1 << 22))
+    hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3(cdiv(p.M, 256) * cdiv(p.N, 256)), dim3(256), 0, s, p);
+  else
+    hipLaunchKernelGGL((fp8_gemm_kernel<128, 128, 2, 2, ACT, CT>), dim3(cdiv(p.M, 128) * cdiv(p.N, 128)), dim3(256), 0, s, p);
+}
+
+template <int ACT>
+void launch_act(const Fp8Gemm& p, int ctype, hipStream_t s) {
+  if (ctype == C_BF16) launch<ACT, C_BF16>(p, s);
+  else if (ctype == C_F16) launch<ACT, C_F16>(p, s);
+  else launch<ACT, C_F32>(p, s);
 }
 
 }  // namespace
@@ -158,8 +393,10 @@ int fp8_gemm_launch(const uint8_t* A, const uint8_t* As, const uint8_t* B, const
                     const float* bias, int M, int N, int nk, long lda, long ldb, int ldsa, int ldsb, int bshift,
                     long ldc, int act, int ctype, hipStream_t s) {
   if (M <= 0 || N <= 0 || nk <= 0) return 0;
-  const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, lda, ldb, ldsa, ldsb, bshift, ldc, act, ctype};
-  launch<128, 128, 2, 2>(p, s);
+  const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, lda, ldb, ldsa, ldsb, bshift, ldc};
+  if (act == ACT_NONE) launch_act<ACT_NONE>(p, ctype, s);
+  else if (act == ACT_RELU) launch_act<ACT_RELU>(p, ctype, s);
+  else launch_act<ACT_SILU>(p, ctype, s);
   HIP_CHECK_LAUNCH();
   return 0;
 }

@@ -521,7 +521,7 @@ def test_fp8_blocks_refuses():
 # ---------------------------------------------------------------------------
 SHAPES = [(1, 1, 1), (1, 130, 256), (2, 16, 640), (16, 33, 1281), (17, 1000, 1280), (33, 64, 2048), (65, 200, 129), (64, 513, 4096),
           (129, 257, 1000), (133, 1000, 1280), (300, 300, 896), (128, 1024, 128), (1000, 120, 512), (515, 1030, 1152),
-          (0, 8, 128), (3, 2, 8192)]
+          (0, 8, 128), (3, 2, 8192), (512, 512, 128), (769, 515, 300), (520, 1025, 1664)]
 
 
 @pytest.mark.parametrize("dev", DEVICES)
