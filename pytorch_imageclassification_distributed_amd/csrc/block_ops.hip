@@ -60,6 +60,47 @@ DEVI void store8(T* p, int valid, const float* f) {
   }
 }
 
+// 8 elements as loaded (half the registers of their float values in a 16-bit type)
+template <typename T>
+struct Raw8 {
+  static constexpr int W = (int)sizeof(T) * 2;
+  uint32_t w[W];
+  DEVI float get(int k) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+    else if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k >> 1] >> (16 * (k & 1))));
+  }
+  // forget that the float values are known: they are made again where they are used next, not kept in registers
+  DEVI void launder() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+
+template <typename T, bool VEC>
+DEVI Raw8<T> raw8(const T* p, int valid) {
+  Raw8<T> v;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int i = 0; i < Raw8<T>::W; i += 4) {
+      uint4 u = make_uint4(0u, 0u, 0u, 0u);
+      if (valid > 0) u = ((const uint4*)p)[i >> 2];
+      v.w[i] = u.x; v.w[i + 1] = u.y; v.w[i + 2] = u.z; v.w[i + 3] = u.w;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v.w[k] = k < valid ? __float_as_uint(p[k]) : 0u;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t lo = 2 * k < valid ? __builtin_bit_cast(uint16_t, p[2 * k]) : 0u;
+      const uint32_t hi = 2 * k + 1 < valid ? __builtin_bit_cast(uint16_t, p[2 * k + 1]) : 0u;
+      v.w[k] = lo | hi << 16;
+    }
+  }
+  return v;
+}
+
 // ---- dropout ----
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", SC 2011): the counter
 // is (element / 8, offset), the key the seed, so element n's number depends on nothing but (n, seed, offset) and the
@@ -190,7 +231,7 @@ DEVI float block_max(const float* f) {
 }
 
 // ---- root-mean-square norm ----
-// sum over the TPR threads of a row (256-thread blocks hold 256 / TPR rows)
+// sum over the TPR threads of a row
 template <int TPR>
 DEVI float row_sum(float v, float* red) {
   v = wave_sum(v);
@@ -206,7 +247,7 @@ DEVI float row_sum(float v, float* red) {
   return v;
 }
 
-constexpr int nthreads(int tpr) { return tpr < 256 ? 256 : tpr; }
+constexpr int nthreads(int tpr) { return tpr == 64 ? 256 : tpr; }  // one row a block where a row needs several waves
 
 // h = res + drop(x), rounded to T (what backward reads); y = h * rsqrt(mean h^2 + eps) * w.  A row stays in registers
 // between the two (V vectors a lane), so x, res are read and h, y written once.
@@ -278,7 +319,8 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_fwd_kernel(const T* __restr
 }
 
 // dh = r (dy w - h r^2 mean(dy w h)) (+ dh_out); dx = drop(dh); a block walks rows and keeps its part of
-// dw = sum_rows dy h r in registers: part[block][N], added up by rows_sum_kernel in a fixed order
+// dw = sum_rows dy h r in registers: part[block][N], added up by rows_sum_kernel in a fixed order.  A row's three
+// inputs are all asked for before the first is used, and stay in their own type until then.
 template <typename T, int TPR, int V, bool VEC, bool DROP>
 __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ h,
                                                                 const T* __restrict__ dh_out,
@@ -297,44 +339,64 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restr
   for (int j = 0; j < V; ++j)
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[j][k] = 0.f;
+  constexpr bool GREG = TPR < 1024;  // the weights stay in registers over the rows where there is room for them
+  float gw[GREG ? V : 1][8];
+  auto weights = [&](int j, float* g) {
+    const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
+    if (w != nullptr) load8<float, VEC>(w + c, valid, g);
+    else
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = 1.f;
+  };
+  if constexpr (GREG)
+#pragma unroll
+    for (int j = 0; j < V; ++j) weights(j, gw[j]);
   for (long row = (long)blockIdx.x * RPB + sub; row < rows; row += (long)gridDim.x * RPB) {
     const long base = row * N;
-    const float inv = rstd[row];
-    float a[V][8], b[V][8];
-    float s = 0.f;
+    Raw8<T> ra[V], rb[V], rc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-      load8<T, VEC>(dy + base + c, valid, a[j]);
-      load8<T, VEC>(h + base + c, valid, b[j]);
+      ra[j] = raw8<T, VEC>(dy + base + c, valid);
+      rb[j] = raw8<T, VEC>(h + base + c, valid);
+    }
+    if (dh_out != nullptr) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) dw[j][k] += a[j][k] * b[j][k] * inv;
-      if (w != nullptr) {
-        float g[8];
-        load8<float, VEC>(w + c, valid, g);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) a[j][k] *= g[k];
+      for (int j = 0; j < V; ++j) {
+        const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
+        rc[j] = raw8<T, VEC>(dh_out + base + c, valid);
       }
+    }
+    const float inv = rstd[row];
+    float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s += a[j][k] * b[j][k];
+    for (int j = 0; j < V; ++j) {
+      if constexpr (!GREG) weights(j, gw[0]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float p = ra[j].get(k) * rb[j].get(k);
+        dw[j][k] += p * inv;
+        s += p * gw[GREG ? j : 0][k];
+      }
+      ra[j].launder();
+      rb[j].launder();
     }
     s = row_sum<TPR>(s, red);
     const float m = s * inv * inv / (float)N;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
+      float o[8];
+      if constexpr (!GREG) weights(j, gw[0]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) a[j][k] = inv * (a[j][k] - b[j][k] * m);
-      if (dh_out != nullptr) {
-        float g[8];
-        load8<T, VEC>(dh_out + base + c, valid, g);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) a[j][k] += g[k];
+      for (int k = 0; k < 8; ++k) {
+        o[k] = inv * (ra[j].get(k) * gw[GREG ? j : 0][k] - rb[j].get(k) * m);
+        if (dh_out != nullptr) o[k] += rc[j].get(k);
       }
-      if (dres != nullptr) store8<T, VEC>(dres + base + c, valid, a[j]);
+      if (dres != nullptr) store8<T, VEC>(dres + base + c, valid, o);
       if constexpr (DROP)
-        if (valid > 0) drop8<VEC>(d, seed, offset, base + c, a[j]);
-      if (dx != nullptr) store8<T, VEC>(dx + base + c, valid, a[j]);
+        if (valid > 0) drop8<VEC>(d, seed, offset, base + c, o);
+      if (dx != nullptr) store8<T, VEC>(dx + base + c, valid, o);
     }
   }
   if (part == nullptr) return;
@@ -360,17 +422,42 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restr
   }
 }
 
-// out[c] = sum_i part[i][c] in a fixed order: 64 columns x 4 row lanes a block
-__global__ __launch_bounds__(256) void rows_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int G,
-                                                       int N) {
-  __shared__ float red[4][64];
-  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
-  float s = 0.f;
-  if (c < N)
-    for (int i = r; i < G; i += 4) s += part[(long)i * N + c];
-  red[r][threadIdx.x & 63] = s;
+// out[c] = sum_i part[i][c] in a fixed order.  A block owns 64 columns: 16 lanes of 4 columns x 64 row lanes, so that
+// the few hundred partial rows of a column are read in a handful of loads in flight at once (a block of 4 row lanes
+// took 75 us for 1024 x 2048 partials: one load after the other).
+template <bool VEC>
+__global__ __launch_bounds__(1024) void rows_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int G,
+                                                        int N) {
+  __shared__ float red[64][65];
+  __shared__ float fin[4][64];
+  const int lc = threadIdx.x & 15, lr = threadIdx.x >> 4;
+  const int c = blockIdx.x * 64 + lc * 4;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = lr; i < G; i += 64) {
+    if constexpr (VEC) {
+      if (c < N) {
+        const float4 v = *(const float4*)(part + (long)i * N + c);
+        s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k] += c + k < N ? part[(long)i * N + c + k] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) red[lr][lc * 4 + k] = s[k];
   __syncthreads();
-  if (r == 0 && c < N) out[c] = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+  if (threadIdx.x < 256) {
+    const int col = threadIdx.x & 63, q = threadIdx.x >> 6;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v += red[q * 16 + i][col];
+    fin[q][col] = v;
+  }
+  __syncthreads();
+  const int cc = blockIdx.x * 64 + threadIdx.x;
+  if (threadIdx.x < 64 && cc < N) out[cc] = (fin[0][threadIdx.x] + fin[1][threadIdx.x]) + (fin[2][threadIdx.x] + fin[3][threadIdx.x]);
 }
 
 // ---- quantisation ----
@@ -518,15 +605,28 @@ int dropout_counter_launch(const void* x, const void* res, void* y, long n, int 
   return 0;
 }
 
-// threads a row and vectors a thread: the smallest that hold the row
-#define RMS_SHAPE(N, ...)                                                              \
-  if (N <= 512) { constexpr int TPR = 64, V = 1; __VA_ARGS__; }                        \
-  else if (N <= 1024) { constexpr int TPR = 64, V = 2; __VA_ARGS__; }                  \
-  else if (N <= 2048) { constexpr int TPR = 64, V = 4; __VA_ARGS__; }                  \
-  else if (N <= 4096) { constexpr int TPR = 256, V = 2; __VA_ARGS__; }                 \
-  else if (N <= 8192) { constexpr int TPR = 256, V = 4; __VA_ARGS__; }                 \
-  else if (N <= 16384) { constexpr int TPR = 1024, V = 2; __VA_ARGS__; }               \
-  else if (N <= 32768) { constexpr int TPR = 1024, V = 4; __VA_ARGS__; }               \
+// Threads a row and vectors a thread, the smallest that hold the row.  Forward: two vectors a thread, few registers
+// and 8 waves a SIMD (8192 x 2048 with dropout 27.5 us against 28.7 with four vectors, 16384 x 8192 184 against 192).
+// Backward: four, where a row's partial dw sits in fewer threads and a row of 2048 needs no barrier (31.3 us against
+// 44.0, and 210 against 220).
+#define RMS_CASE(LIMIT, T_, V_, ...) if (N <= LIMIT) { constexpr int TPR = T_, V = V_; __VA_ARGS__; }
+#define RMS_FWD_SHAPE(N, ...)                      \
+  RMS_CASE(512, 64, 1, __VA_ARGS__)                \
+  else RMS_CASE(1024, 64, 2, __VA_ARGS__)          \
+  else RMS_CASE(2048, 128, 2, __VA_ARGS__)         \
+  else RMS_CASE(4096, 256, 2, __VA_ARGS__)         \
+  else RMS_CASE(8192, 512, 2, __VA_ARGS__)         \
+  else RMS_CASE(16384, 1024, 2, __VA_ARGS__)       \
+  else RMS_CASE(32768, 1024, 4, __VA_ARGS__)       \
+  else return (int)hipErrorInvalidValue;
+#define RMS_BWD_SHAPE(N, ...)                      \
+  RMS_CASE(512, 64, 1, __VA_ARGS__)                \
+  else RMS_CASE(1024, 64, 2, __VA_ARGS__)          \
+  else RMS_CASE(2048, 64, 4, __VA_ARGS__)          \
+  else RMS_CASE(4096, 256, 2, __VA_ARGS__)         \
+  else RMS_CASE(8192, 256, 4, __VA_ARGS__)         \
+  else RMS_CASE(16384, 1024, 2, __VA_ARGS__)       \
+  else RMS_CASE(32768, 1024, 4, __VA_ARGS__)       \
   else return (int)hipErrorInvalidValue;
 
 int rms_max_cols() { return 32768; }
@@ -537,7 +637,7 @@ int rms_fwd_launch(const void* x, const void* res, const float* w, void* h, void
   if (rows <= 0) return 0;
   const Drop d = make_drop(state, seed, offset, t);
   BLOCK_TYPE(type, {
-    RMS_SHAPE(N, {
+    RMS_FWD_SHAPE(N, {
       constexpr int NT = nthreads(TPR);
       const dim3 grid((unsigned)((rows + NT / TPR - 1) / (NT / TPR)));
       auto go = [&](auto vec, auto drop, auto fp8) {
@@ -561,10 +661,11 @@ int rms_fwd_launch(const void* x, const void* res, const float* w, void* h, void
   return 0;
 }
 
-// blocks of a backward launch = rows of the dw partials
+// blocks of a backward launch = rows of the dw partials.  512 keep the chip busy; 1024 cost 3 us more in the sum over
+// the partials than they save here (8192 x 2048)
 int rms_bwd_blocks(long rows, int N) {
   const long per = N <= 2048 ? 4 : 1, need = (rows + per - 1) / per;
-  return (int)(need < 1 ? 1 : need < 1024 ? need : 1024);
+  return (int)(need < 1 ? 1 : need < 512 ? need : 512);
 }
 
 int rms_bwd_launch(const void* dy, const void* h, const void* dh, const float* w, const float* rstd, void* dx,
@@ -573,7 +674,7 @@ int rms_bwd_launch(const void* dy, const void* h, const void* dh, const float* w
   if (rows <= 0) return 0;
   const Drop d = make_drop(state, seed, offset, t);
   BLOCK_TYPE(type, {
-    RMS_SHAPE(N, {
+    RMS_BWD_SHAPE(N, {
       constexpr int NT = nthreads(TPR);
       auto go = [&](auto vec, auto drop) {
         hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, V, decltype(vec)::value, decltype(drop)::value>), dim3(blocks),
@@ -592,7 +693,8 @@ int rms_bwd_launch(const void* dy, const void* h, const void* dh, const float* w
 
 int rows_sum_launch(const float* part, float* out, int G, int N, hipStream_t s) {
   if (N <= 0) return 0;
-  hipLaunchKernelGGL(rows_sum_kernel, dim3(cdiv(N, 64)), dim3(256), 0, s, part, out, G, N);
+  if (N % 4 == 0) hipLaunchKernelGGL(rows_sum_kernel<true>, dim3(cdiv(N, 64)), dim3(1024), 0, s, part, out, G, N);
+  else hipLaunchKernelGGL(rows_sum_kernel<false>, dim3(cdiv(N, 64)), dim3(1024), 0, s, part, out, G, N);
   HIP_CHECK_LAUNCH();
   return 0;
 }
