@@ -1,10 +1,16 @@
-// Bindings of the pre-norm 8-bit linear block (block_ops.hip, fp8_gemm.hip): every argument a kernel's indexing relies
-// on is checked here, the launch goes to the current stream of the tensors' own device, and nothing is allocated.
+// The pre-norm 8-bit linear block (block_ops.hip, fp8_gemm.hip) as autograd operators.  Every argument a kernel's
+// indexing relies on is checked here, the launch goes to the current stream of the tensors' own device, and outputs and
+// workspaces come from the caching allocator (they live as long as the call, or as what it saves for backward).
+//
+// The autograd nodes are C++: a small call is bound by the host, and a Python node costs it twice the time of one of
+// torch's own (4 x 2048 dropout, forward and backward: 70 us with a Python node, 46 us for torch's product).
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <optional>
 
 using at::Tensor;
@@ -26,6 +32,10 @@ int quant_rows_launch(const void*, const void*, uint8_t*, uint8_t*, bf16_t*, flo
 int quant_tiles_launch(const void*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, int, int, long, int, long, int, int,
                        hipStream_t);
 int dequant_launch(const uint8_t*, const uint8_t*, void*, long, int, long, int, int, int, hipStream_t);
+int zero_f32_launch(float*, long, hipStream_t);
+// bindings.cpp: dW[Cout][Cin] += dY[M][Cout]^T X[M][Cin], bf16, Cout and Cin multiples of 8
+void dense_wgrad(Tensor dY, Tensor X, Tensor dW, int M, int Cout, int Cin, int k_per_split, int splits, Tensor zero,
+                 int stages, std::optional<Tensor> ws);
 int fp8_gemm_launch(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, const float*, int, int, int,
                     long, long, int, int, int, long, int, int, hipStream_t);
 
@@ -232,22 +242,349 @@ void fp8_gemm(Tensor a, Tensor as, Tensor b, Tensor bs, Tensor c, OT bias, int64
      "matmul_fp8");
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// operators
+// ---------------------------------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// row-major and 16-byte aligned (the kernels move whole 16-byte vectors); a copy where it is not
+Tensor dense16(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
+}
+OT dense16(const OT& t) { return t.has_value() && t->defined() ? OT(dense16(*t)) : OT(); }
+OT f32(const OT& t) { return t.has_value() && t->defined() ? OT(dense16(t->detach().to(at::kFloat))) : OT(); }
+OT some(const Tensor& t) { return t.defined() ? OT(t) : OT(); }
+bool has(const OT& t) { return t.has_value() && t->defined(); }
+Tensor or_undefined(const OT& t) { return has(t) ? *t : Tensor(); }
+bool wants(const OT& t) { return has(t) && t->requires_grad(); }
+
+Tensor fresh(at::IntArrayRef size, const Tensor& like, at::ScalarType st) { return at::empty(size, like.options().dtype(st)); }
+
+struct Blocks {
+  Tensor q, sc;
+};
+Blocks empty_blocks(int64_t rows, int64_t cols, int64_t tile, const Tensor& like) {
+  const int64_t nb = (cols + 127) / 128;
+  return {fresh({rows, nb * 128}, like, at::kFloat8_e4m3fn), fresh({(rows + tile - 1) / tile, (nb + 3) / 4 * 4}, like, at::kByte)};
+}
+
+// A Python callable that hands out the tensor for a parameter's float32 gradient (its gradient-arena slot)
+struct Slot : torch::CustomClassHolder {
+  py::object fn;
+  explicit Slot(py::object f) : fn(std::move(f)) {}
+  ~Slot() override {
+    py::gil_scoped_acquire gil;
+    fn = py::object();
+  }
+};
+c10::IValue slot_value(const py::object& fn) {
+  if (fn.is_none()) return c10::IValue();
+  return c10::IValue::make_capsule(c10::make_intrusive<Slot>(fn));
+}
+Tensor slot_or_empty(const c10::IValue& v, at::IntArrayRef size, const Tensor& like) {
+  if (v.isNone()) return fresh(size, like, at::kFloat);
+  auto slot = c10::static_intrusive_pointer_cast<Slot>(v.toCapsule());
+  py::gil_scoped_acquire gil;
+  return py::cast<Tensor>(slot->fn());
+}
+
+// The kernels' gradients have no second derivative: differentiating them again raises
+variable_list no_second(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (auto& g : grads)
+    if (g.defined()) in.push_back(g.detach().requires_grad_(true));
+  auto err = std::make_shared<torch::autograd::DelayedError>(
+      "the gradients of the dropout / RMS norm / 8-bit linear operators cannot be differentiated again", (int64_t)in.size());
+  variable_list out = (*err)(std::move(in));
+  size_t i = 0;
+  for (auto& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
+// drop arguments that travel through the nodes: threshold, seed, offset (64-bit patterns), and the device state
+struct DropArgs {
+  int64_t t;
+  uint64_t seed, offset;
+  void save(AutogradContext* ctx) const {
+    ctx->saved_data["t"] = t;
+    ctx->saved_data["seed"] = (int64_t)seed;
+    ctx->saved_data["offset"] = (int64_t)offset;
+  }
+  static DropArgs load(AutogradContext* ctx) {
+    return {ctx->saved_data["t"].toInt(), (uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt()};
+  }
+};
+
+Tensor drop_forward(const Tensor& x, const OT& residual, const OT& state, const DropArgs& d) {
+  Tensor xd = dense16(x), y = at::empty_like(xd);
+  dropout_counter(xd, dense16(residual), y, state, d.seed, d.offset, (int)d.t);
+  return y;
+}
+
+struct DropoutCounterNode : torch::autograd::Function<DropoutCounterNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OT& residual, const OT& state, int64_t t,
+                        int64_t seed, int64_t offset) {
+    const DropArgs d{t, (uint64_t)seed, (uint64_t)offset};
+    ctx->save_for_backward({or_undefined(state)});
+    d.save(ctx);
+    ctx->saved_data["res"] = has(residual);
+    return drop_forward(x, residual, state, d);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const OT state = some(ctx->get_saved_variables()[0]);
+    Tensor dx;
+    if (ctx->needs_input_grad(0)) dx = drop_forward(g[0].detach(), OT(), state, DropArgs::load(ctx));
+    variable_list out = no_second({dx});
+    return {out[0], ctx->saved_data["res"].toBool() ? g[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor op_dropout_counter(const Tensor& x, const OT& residual, const OT& state, uint64_t seed, uint64_t offset, int64_t t) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual)))
+    return drop_forward(x.detach(), residual, state, {t, seed, offset});
+  return DropoutCounterNode::apply(x, residual, state, t, (int64_t)seed, (int64_t)offset);
+}
+
+// y (and h): one pass over x and residual; h and one float a row are kept for the backward pass, which makes the dropout
+// mask again
+struct RmsOut {
+  Tensor y, h, w, rstd;  // h undefined where it equals x
+};
+RmsOut rms_forward(const Tensor& x, const OT& residual, const OT& weight, const OT& state, const DropArgs& d, double eps,
+                   bool need) {
+  const int64_t n = x.size(-1), rows = x.numel() / n;
+  RmsOut o;
+  o.y = at::empty_like(x);
+  if (has(residual) || (d.t > 0 && need)) o.h = at::empty_like(x);
+  if (need) o.rstd = fresh({rows}, x, at::kFloat);
+  const OT w = f32(weight);
+  o.w = or_undefined(w);
+  rms_fwd(x, dense16(residual), w, some(o.h), o.y, some(o.rstd), rows, n, eps, state, d.seed, d.offset, (int)d.t);
+  return o;
+}
+
+struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_, const OT& residual, const OT& weight,
+                               const OT& state, int64_t t, int64_t seed, int64_t offset, double eps, c10::IValue slot) {
+    const DropArgs d{t, (uint64_t)seed, (uint64_t)offset};
+    const Tensor x = dense16(x_);
+    RmsOut o = rms_forward(x, residual, weight, state, d, eps, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({o.h.defined() ? o.h : x, o.w, o.rstd, or_undefined(state)});
+    d.save(ctx);
+    ctx->saved_data["res"] = has(residual);
+    ctx->saved_data["wtype"] = has(weight) ? (int64_t)weight->scalar_type() : (int64_t)-1;
+    ctx->saved_data["slot"] = std::move(slot);
+    if (has(residual)) return {o.y, o.h};
+    return {o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &h = s[0], &rstd = s[2];
+    const OT w = some(s[1]), state = some(s[3]);
+    const DropArgs d = DropArgs::load(ctx);
+    const int64_t n = h.size(-1), rows = h.numel() / n;
+    const bool res = ctx->saved_data["res"].toBool();
+    // (needs_input_grad counts the defined tensors)
+    const bool nx = ctx->needs_input_grad(0), nr = res && ctx->needs_input_grad(1), nw = w.has_value() && ctx->needs_input_grad(1 + res);
+    const Tensor dy = g[0].defined() ? dense16(g[0].detach()) : at::zeros_like(h);
+    const OT dh = res && g[1].defined() ? OT(dense16(g[1].detach())) : OT();
+    Tensor dx, dres, part, dw;
+    const bool both = nx || !nr;  // without dropout the two gradients are one tensor
+    if (both) dx = at::empty_like(h);
+    if (nr && (d.t > 0 || !both)) dres = at::empty_like(h);
+    if (nw) part = fresh({rms_bwd_blocks(rows, (int)n), n}, h, at::kFloat);
+    rms_bwd(dy, h, dh, w, rstd, some(dx), some(dres), some(part), rows, n, state, d.seed, d.offset, (int)d.t);
+    if (nw) {
+      dw = slot_or_empty(ctx->saved_data["slot"], {n}, h);
+      rows_sum(part, dw, rows ? part.size(0) : 0, n);
+      const auto wt = (at::ScalarType)ctx->saved_data["wtype"].toInt();
+      if (wt != at::kFloat) dw = dw.to(wt);
+    }
+    variable_list out = no_second({nx ? dx : Tensor(), nr ? (dres.defined() ? dres : dx) : Tensor(), dw});
+    return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// [y] or [y, h]
+std::vector<Tensor> op_rms_norm(const Tensor& x, const OT& residual, const OT& weight, const OT& state, uint64_t seed,
+                                uint64_t offset, int64_t t, double eps, py::object slot) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual) || wants(weight))) {
+    RmsOut o = rms_forward(dense16(x.detach()), residual, weight, state, {t, seed, offset}, eps, false);
+    if (has(residual)) return {o.y, o.h};
+    return {o.y};
+  }
+  return RmsNormNode::apply(x, residual, weight, state, t, (int64_t)seed, (int64_t)offset, eps, slot_value(slot));
+}
+
+// (q, scale, h or None)
+std::tuple<Tensor, Tensor, OT> op_rms_norm_fp8(const Tensor& x_, const OT& residual, const OT& weight, double eps) {
+  const at::NoGradGuard no_grad;
+  const Tensor x = dense16(x_.detach());
+  const int64_t n = x.size(-1), rows = x.numel() / n;
+  Blocks b = empty_blocks(rows, n, 1, x);
+  OT h;
+  if (has(residual)) h = at::empty_like(x);
+  rms_fwd_fp8(x, dense16(residual), f32(weight), h, b.q, b.sc, rows, n, eps);
+  return {b.q, b.sc, h};
+}
+
+std::tuple<Tensor, Tensor> op_quantize_rows(const Tensor& x_) {
+  const Tensor x = dense16(x_.detach());
+  Blocks b = empty_blocks(x.size(0), x.size(1), 1, x);
+  quant_rows(x, OT(), b.q, b.sc, OT(), OT(), x.size(0), x.size(1));
+  return {b.q, b.sc};
+}
+
+std::tuple<Tensor, Tensor> op_quantize_tiles(const Tensor& w_) {
+  const Tensor w = dense16(w_.detach());
+  Blocks b = empty_blocks(w.size(0), w.size(1), 128, w);
+  quant_tiles(w, b.q, b.sc, OT(), OT());
+  return {b.q, b.sc};
+}
+
+Tensor op_matmul(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, const OT& bias, int64_t n, int64_t k,
+                 int64_t btile, int64_t act, at::ScalarType out) {
+  Tensor c = fresh({a.size(0), n}, a, out);
+  fp8_gemm(a, as, b, bs, c, f32(bias), k, btile, (int)act);
+  return c;
+}
+
+// dw[n][k] = sum over the m rows of dy[row][n] x[row][k] on the bf16 weight-gradient kernels (the rows are the pixels of
+// a 1x1 convolution over 1x1 maps).  dy, x: widths rounded up to 8.
+void rows_grad(const Tensor& dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k, const Tensor& zero) {
+  const c10::DeviceGuard guard(dw.device());
+  const int64_t n8 = (n + 7) / 8 * 8, k8 = (k + 7) / 8 * 8;
+  const bool direct = n8 == n && k8 == k;
+  const Tensor out = direct ? dw : fresh({n8, k8}, dw, at::kFloat);
+  ok(zero_f32_launch(out.data_ptr<float>(), out.numel(), stream_of(out)), "zero");
+  if (m > 0) {
+    const int stages = n8 >= 256 && k8 >= 256 ? 7 : 2;
+    const int64_t side = stages == 7 ? 256 : 128;
+    const int64_t rows = n8 > 64 ? side : 64, tiles = ((n8 + rows - 1) / rows) * ((k8 + side - 1) / side);
+    // at most 8 slabs: they are added in one ordered pass
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({8, 512 / tiles, m / 512}));
+    const int64_t kps = ((m + splits - 1) / splits + 63) / 64 * 64;
+    splits = (m + kps - 1) / kps;
+    OT slabs;
+    if (splits > 1) slabs = fresh({splits * n8 * k8}, dw, at::kFloat);
+    dense_wgrad(dy, x, out, (int)m, (int)n8, (int)k8, (int)kps, (int)splits, zero, stages, slabs);
+  }
+  if (!direct) dw.copy_(out.narrow(0, 0, n).narrow(1, 0, k));
+}
+
+// y = act(q(x) q(w)^T + b).  Backward: dx = q(dy) q(w) in 8 bits (the weights' transpose was written beside them; 128 x
+// 128 tiles keep their scale), db in float32, and dw = dy^T x on bf16 operands: weight gradients are summed into float32
+// masters over many steps, and the 8-bit matrix instructions cut their sums at 2^-16 where the bf16 ones keep float32.
+struct LinearOut {
+  Tensor y, xb, wt, wtsc;
+};
+LinearOut linear_forward(const Tensor& x, const Tensor& weight, const OT& bias, int64_t act, bool need_x, bool need_w) {
+  const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+  LinearOut o;
+  Blocks a = empty_blocks(m, k, 1, x), b = empty_blocks(n, k, 128, x);
+  OT copy, wt, wtsc;
+  if (need_w) {
+    o.xb = x;
+    if (x.scalar_type() != at::kBFloat16 || k % 8) {
+      o.xb = fresh({m, (k + 7) / 8 * 8}, x, at::kBFloat16);
+      copy = o.xb;
+    }
+  }
+  quant_rows(x, OT(), a.q, a.sc, copy, OT(), m, k);
+  if (need_x) {
+    Blocks t = empty_blocks(k, n, 128, x);
+    o.wt = t.q; o.wtsc = t.sc;
+    wt = t.q; wtsc = t.sc;
+  }
+  quant_tiles(dense16(weight.detach()), b.q, b.sc, wt, wtsc);
+  o.y = fresh({m, n}, x, x.scalar_type());
+  fp8_gemm(a.q, a.sc, b.q, b.sc, o.y, f32(bias), k, 128, (int)act);
+  return o;
+}
+
+struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weight, const OT& bias, const Tensor& zero,
+                        int64_t act, bool need_x, bool need_w, c10::IValue wslot, c10::IValue bslot) {
+    const Tensor x = dense16(x_);
+    LinearOut o = linear_forward(x, weight, bias, act, need_x, need_w);
+    ctx->save_for_backward({o.xb, o.wt, o.wtsc, act ? o.y : Tensor(), zero});
+    ctx->saved_data["m"] = x.size(0);
+    ctx->saved_data["n"] = weight.size(0);
+    ctx->saved_data["k"] = x.size(1);
+    ctx->saved_data["wtype"] = (int64_t)weight.scalar_type();
+    ctx->saved_data["bias"] = has(bias);
+    ctx->saved_data["btype"] = has(bias) ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat;
+    ctx->saved_data["wslot"] = std::move(wslot);
+    ctx->saved_data["bslot"] = std::move(bslot);
+    return o.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &xb = s[0], &wt = s[1], &wtsc = s[2];
+    const OT y = some(s[3]);
+    const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    const Tensor dy = dense16(g[0].detach());
+    Blocks b;
+    Tensor dyb = dy, part, dx, dw, db;
+    OT copy;
+    if (nx) b = empty_blocks(m, n, 1, dy);
+    if (nw && (dy.scalar_type() != at::kBFloat16 || n % 8 || y.has_value())) {
+      dyb = fresh({m, (n + 7) / 8 * 8}, dy, at::kBFloat16);
+      copy = dyb;
+    }
+    if (nb) {
+      const int64_t c = quant_rows_chunk(m, (int)n);
+      part = fresh({(m + c - 1) / c, n}, dy, at::kFloat);
+    }
+    if (nx || copy.has_value() || nb) quant_rows(dy, y, some(b.q), some(b.sc), copy, some(part), m, n);
+    if (nx) {
+      dx = fresh({m, k}, dy, dy.scalar_type());
+      fp8_gemm(b.q, b.sc, wt, wtsc, dx, OT(), n, 128, 0);
+    }
+    if (nw) {
+      dw = slot_or_empty(ctx->saved_data["wslot"], {n, k}, dy);
+      rows_grad(dyb, xb, dw, m, n, k, s[4]);
+      const auto t = (at::ScalarType)ctx->saved_data["wtype"].toInt();
+      if (t != at::kFloat) dw = dw.to(t);
+    }
+    if (nb) {
+      db = slot_or_empty(ctx->saved_data["bslot"], {n}, dy);
+      rows_sum(part, db, part.size(0), n);
+      const auto t = (at::ScalarType)ctx->saved_data["btype"].toInt();
+      if (t != at::kFloat) db = db.to(t);
+    }
+    variable_list out = no_second({dx, dw, db});
+    return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor op_linear_fp8(const Tensor& x, const Tensor& weight, const OT& bias, const Tensor& zero, int64_t act,
+                     py::object wslot, py::object bslot) {
+  const bool grad = at::GradMode::is_enabled(), nx = grad && x.requires_grad(), nw = grad && weight.requires_grad();
+  if (!(nx || nw || (grad && wants(bias)))) return linear_forward(dense16(x.detach()), weight, bias, act, false, false).y;
+  return LinearFp8Node::apply(x, weight, bias, zero, act, nx, nw, slot_value(wslot), slot_value(bslot));
+}
+
 }  // namespace
 
 void register_block_ops(pybind11::module& m) {
-  m.def("dropout_counter", &dropout_counter);
   m.def("rms_max_cols", &rms_max_cols);
-  m.def("rms_fwd", &rms_fwd);
-  m.def("rms_fwd_fp8", &rms_fwd_fp8);
-  m.def("rms_bwd_blocks", [](int64_t rows, int64_t N) { return rms_bwd_blocks(rows, (int)N); });
-  m.def("rms_bwd", &rms_bwd);
-  m.def("rows_sum", &rows_sum);
-  m.def("quant_rows_groups", [](int64_t M, int64_t N) {
-    const int c = quant_rows_chunk(M, (int)N);
-    return (M + c - 1) / c;
+  m.def("dropout_counter", &op_dropout_counter);
+  m.def("rms_norm", &op_rms_norm);
+  m.def("rms_norm_fp8", &op_rms_norm_fp8);
+  m.def("quantize_fp8_rows", &op_quantize_rows);
+  m.def("quantize_fp8_tiles", &op_quantize_tiles);
+  m.def("dequantize_fp8", &fp8_dequant);
+  m.def("matmul_fp8", [](const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, const OT& bias, int64_t n,
+                         int64_t k, int64_t btile, int64_t act, py::object dtype) {
+    return op_matmul(a, as, b, bs, bias, n, k, btile, act, torch::python::detail::py_object_to_dtype(dtype));
   });
-  m.def("quant_rows", &quant_rows);
-  m.def("quant_tiles", &quant_tiles);
-  m.def("fp8_dequant", &fp8_dequant);
-  m.def("fp8_gemm", &fp8_gemm);
+  m.def("linear_fp8", &op_linear_fp8);
 }

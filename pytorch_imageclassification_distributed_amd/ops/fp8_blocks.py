@@ -55,6 +55,13 @@ class Fp8Blocks:
             raise ValueError(f"Fp8Blocks: q on {q.device}, scale on {scale.device}")
         self.q, self.scale, self.shape, self.tile = q, scale, (rows, cols), tile
 
+    @classmethod
+    def _made(cls, q, scale, shape, tile):
+        """Blocks that a quantiser of this package has just laid out (nothing left to check)."""
+        self = cls.__new__(cls)
+        self.q, self.scale, self.shape, self.tile = q, scale, shape, tile
+        return self
+
     @property
     def device(self):
         return self.q.device

@@ -791,6 +791,16 @@ def test_block_gradients_land_in_the_arena():
         arena.detach_params()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_derivatives_are_refused(dev):
+    x = rand((4, 64), torch.float32, dev, 170).requires_grad_(True)
+    norm, lin = nn.RMSNorm(64).to(dev), nn.Linear(64, 8).to(dev)
+    for f in (lambda: Fx.rms_norm(x, norm), lambda: Fx.linear_fp8(x, lin)):
+        (g,) = torch.autograd.grad(f().square().sum(), (x,), create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
 @gpu
 def test_block_facade_and_missing_fallback():
     """The op layer's HIP part owns every name, and the operators run its kernels for GPU tensors (the torch backend gives
