@@ -33,6 +33,7 @@ int quant_tiles_launch(const void*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, int,
                        hipStream_t);
 int dequant_launch(const uint8_t*, const uint8_t*, void*, long, int, long, int, int, int, hipStream_t);
 int zero_f32_launch(float*, long, hipStream_t);
+void fp8_gemm_force(int);
 // bindings.cpp: dW[Cout][Cin] += dY[M][Cout]^T X[M][Cin], bf16, Cout and Cin multiples of 8
 void dense_wgrad(Tensor dY, Tensor X, Tensor dW, int M, int Cout, int Cin, int k_per_split, int splits, Tensor zero,
                  int stages, std::optional<Tensor> ws);
@@ -587,4 +588,5 @@ void register_block_ops(pybind11::module& m) {
     return op_matmul(a, as, b, bs, bias, n, k, btile, act, torch::python::detail::py_object_to_dtype(dtype));
   });
   m.def("linear_fp8", &op_linear_fp8);
+  m.def("fp8_gemm_force", &fp8_gemm_force);
 }

@@ -39,45 +39,91 @@ DEVI uint32_t pack_c(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
 }
 
-// BM x BN tile on WM x WN waves, two LDS stages of one k-step each filled by LDS-DMA.  Rows past M or N read the last
-// row again (their results are not stored).
-template <int BM, int BN, int WM, int WN, int ACT, int CT>
+DEVI void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, int soff, char* lds_wave_base) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 16, voff, soff, 0, 0);
+}
+
+DEVI i32x8 frag8(const char* lo, const char* hi) {
+  const int4 l = *(const int4*)lo, h = *(const int4*)hi;
+  return (i32x8){l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
+}
+
+// four consecutive outputs of one row
+template <int ACT, int CT>
+DEVI void store4(const Fp8Gemm& p, int m, int n, const f32x4& v, const float* bias) {
+  if (m >= p.M || n >= p.N) return;
+  float o[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = apply_act(v[r] + bias[r], ACT);
+  const long i = (long)m * p.ldc + n;
+  if ((p.ldc & 3) == 0 && n + 4 <= p.N) {
+    if constexpr (CT == C_F32) *(float4*)((float*)p.C + i) = make_float4(o[0], o[1], o[2], o[3]);
+    else *(uint2*)((uint16_t*)p.C + i) = make_uint2(pack_c<CT>(o[0], o[1]), pack_c<CT>(o[2], o[3]));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) store_c<CT>(p, i + r, o[r]);
+  }
+}
+
+DEVI void bias4(const Fp8Gemm& p, int n, float* b) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) b[r] = p.bias != nullptr && n + r < p.N ? p.bias[n + r] : 0.f;
+}
+
+// BM x BN tile on WM x WN waves, a ring of S LDS stages of one k-step each filled by LDS-DMA, S - 1 tiles in flight.
+// Rows past the end read zeros (past the buffer resource).  Each stage is an array of its own: hipcc makes an LDS read
+// wait for every LDS-DMA that may write what it reads, and tells them apart by the array alone.
+template <int BM, int BN, int WM, int WN, int S, int ACT, int CT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p) {
   constexpr int NW = WM * WN;
   constexpr int WTM = BM / WM, WTN = BN / WN, RM = WTM / 16, RN = WTN / 16;
-  constexpr int AL = BM / 8 / NW, BL = BN / 8 / NW;
+  constexpr int AL = BM / 8 / NW, BL = BN / 8 / NW, LPS = AL + BL;
   constexpr int STAGE = (BM + BN) * 128;
   static_assert(AL * 8 * NW == BM && BL * 8 * NW == BN, "loader mapping");
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  static_assert(S == 2 || S == 4, "ring depth");
+  __shared__ __attribute__((aligned(16))) char s0[STAGE];
+  __shared__ __attribute__((aligned(16))) char s1[STAGE];
+  __shared__ __attribute__((aligned(16))) char s2[S == 4 ? STAGE : 16];
+  __shared__ __attribute__((aligned(16))) char s3[S == 4 ? STAGE : 16];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid / WN, wn = wid % WN;
   const int gm = (p.M + BM - 1) / BM, gn = (p.N + BN - 1) / BN;
   const int lin = xcd_remap(blockIdx.x, gm * gn);
-  const int bm = lin / gn, bn = lin - bm * gn;
-  const int m0 = bm * BM, n0 = bn * BN;
+  const int m0 = __builtin_amdgcn_readfirstlane(lin / gn * BM), n0 = __builtin_amdgcn_readfirstlane(lin % gn * BN);
 
   const int lrow = lane >> 3, pch = lane & 7;
-  const uint8_t* srca[AL];
-  const uint8_t* srcb[BL];
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.A + (long)m0 * p.lda, (long)(p.M - m0) * p.lda);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.B + (long)n0 * p.ldb, (long)(p.N - n0) * p.ldb);
+  const __amdgpu_buffer_rsrc_t rz = make_rsrc(p.A, 0);
+  unsigned va[AL], vb[BL];
 #pragma unroll
   for (int i = 0; i < AL; ++i) {
     const int row = wid * (BM / NW) + i * 8 + lrow;
-    srca[i] = p.A + (long)min(m0 + row, p.M - 1) * p.lda + (pch ^ ((row >> 1) & 7)) * 16;
+    va[i] = (unsigned)(row * (int)p.lda + (pch ^ ((row >> 1) & 7)) * 16);
   }
 #pragma unroll
   for (int i = 0; i < BL; ++i) {
     const int row = wid * (BN / NW) + i * 8 + lrow;
-    srcb[i] = p.B + (long)min(n0 + row, p.N - 1) * p.ldb + (pch ^ ((row >> 1) & 7)) * 16;
+    vb[i] = (unsigned)(row * (int)p.ldb + (pch ^ ((row >> 1) & 7)) * 16);
   }
-  auto issue = [&](int kt, int buf) {
-    char* sa = smem + buf * STAGE;
-    char* sb = sa + BM * 128;
+  const int nk = p.nk;
+  // every step issues its pieces (past the last tile from an empty resource), so the counted waits are constant
+  auto issue = [&](int kt, char* buf) __attribute__((always_inline)) {
+    const bool live = kt < nk;
 #pragma unroll
-    for (int i = 0; i < AL; ++i) glds16(srca[i] + (long)kt * 128, sa + (wid * (BM / NW) + i * 8) * 128);
+    for (int i = 0; i < AL; ++i) dma16(live ? ra : rz, va[i], kt * 128, buf + (wid * (BM / NW) + i * 8) * 128);
 #pragma unroll
-    for (int i = 0; i < BL; ++i) glds16(srcb[i] + (long)kt * 128, sb + (wid * (BN / NW) + i * 8) * 128);
+    for (int i = 0; i < BL; ++i) dma16(live ? rb : rz, vb[i], kt * 128, buf + BM * 128 + (wid * (BN / NW) + i * 8) * 128);
+  };
+  auto stage = [&](auto c) __attribute__((always_inline)) -> char* {
+    constexpr int U = decltype(c)::value % S;
+    if constexpr (U == 0) return s0;
+    else if constexpr (U == 1) return s1;
+    else if constexpr (U == 2) return s2;
+    else return s3;
   };
 
   const int fr = lane & 15, fq = lane >> 4;
@@ -102,34 +148,32 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
 #pragma unroll
     for (int j = 0; j < RN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-  issue(0, 0);
-  for (int kt = 0; kt < p.nk; ++kt) {
-    wait_vmcnt<0>();
+  // step kt = S n + U: tile kt has landed (S - 2 younger ones are in flight), every wave has left step kt - 1, whose
+  // stage takes tile kt + S - 1
+  auto step = [&](auto c, int kt) __attribute__((always_inline)) {
+    constexpr int U = decltype(c)::value;
+    wait_vmcnt<(S - 2) * LPS>();
     __builtin_amdgcn_s_barrier();
-    if (kt + 1 < p.nk) issue(kt + 1, (kt + 1) & 1);
+    issue(kt + S - 1, stage(std::integral_constant<int, U + S - 1>{}));
     if ((kt & 3) == 0) {
-      const int nxt = min((kt >> 2) + 1, (p.nk - 1) >> 2);
+      const int nxt = min((kt >> 2) + 1, (nk - 1) >> 2);
 #pragma unroll
       for (int i = 0; i < RM; ++i) { sx[i] = nx[i]; nx[i] = ssa[i][nxt]; }
 #pragma unroll
       for (int j = 0; j < RN; ++j) { sw[j] = nw[j]; nw[j] = ssb[j][nxt]; }
     }
-    const char* sa = smem + (kt & 1) * STAGE;
+    const char* sa = stage(c);
     const char* sb = sa + BM * 128;
     i32x8 xa[RM], wb[RN];
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
       const int row = wm * WTM + i * 16 + fr;
-      const int4 lo = *(const int4*)(sa + swz(row, fq));
-      const int4 hi = *(const int4*)(sa + swz(row, fq + 4));
-      xa[i] = (i32x8){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      xa[i] = frag8(sa + swz(row, fq), sa + swz(row, fq + 4));
     }
 #pragma unroll
     for (int j = 0; j < RN; ++j) {
       const int row = wn * WTN + j * 16 + fr;
-      const int4 lo = *(const int4*)(sb + swz(row, fq));
-      const int4 hi = *(const int4*)(sb + swz(row, fq + 4));
-      wb[j] = (i32x8){lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      wb[j] = frag8(sb + swz(row, fq), sb + swz(row, fq + 4));
     }
 #pragma unroll
     for (int i = 0; i < RM; ++i)
@@ -141,20 +185,85 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
     for (int i = 0; i < RM; ++i) sx[i] >>= 8;
 #pragma unroll
     for (int j = 0; j < RN; ++j) sw[j] >>= 8;
+  };
+  issue(0, s0);
+  if constexpr (S == 4) {
+    issue(1, s1);
+    issue(2, s2);
   }
+  for (int kt = 0;;) {
+    step(std::integral_constant<int, 0>{}, kt);
+    if (++kt >= nk) break;
+    step(std::integral_constant<int, 1>{}, kt);
+    if (++kt >= nk) break;
+    if constexpr (S == 4) {
+      step(std::integral_constant<int, 2>{}, kt);
+      if (++kt >= nk) break;
+      step(std::integral_constant<int, 3>{}, kt);
+      if (++kt >= nk) break;
+    }
+  }
+  wait_vmcnt<0>();
   // acc[i][j][r]: row wm * WTM + 16 i + fr, column wn * WTN + 16 j + 4 fq + r of the tile
 #pragma unroll
-  for (int i = 0; i < RM; ++i) {
-    const int m = m0 + wm * WTM + i * 16 + fr;
-    if (m >= p.M) continue;
+  for (int j = 0; j < RN; ++j) {
+    const int n = n0 + wn * WTN + j * 16 + fq * 4;
+    float bias[4];
+    bias4(p, n, bias);
 #pragma unroll
-    for (int j = 0; j < RN; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = n0 + wn * WTN + j * 16 + fq * 4 + r;
-        if (n < p.N) store_c<CT>(p, (long)m * p.ldc + n, apply_act(acc[i][j][r] + (p.bias ? p.bias[n] : 0.f), ACT));
-      }
+    for (int i = 0; i < RM; ++i) store4<ACT, CT>(p, m0 + wm * WTM + i * 16 + fr, n, acc[i][j], bias);
   }
+}
+
+// ---- few rows ----
+// 16 RM rows x 16 columns a block, its 8 waves each a share of the k-steps, their partial sums joined through LDS in a
+// fixed order.  The weights' bytes bound it, so they go from memory straight into the fragments (16 rows x 128 whole
+// bytes a wave and k-step; no LDS, no barrier before the join), and a launch has N / 16 x 8 waves to keep them coming.
+template <int RM, int ACT, int CT>
+__global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
+  constexpr int W = 8;
+  __shared__ f32x4 part[W][RM][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fq = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * RM;
+  const int nk = p.nk, k0 = wid * nk / W, k1 = (wid + 1) * nk / W;
+  const uint8_t* B = p.B + (long)min(n0 + fr, p.N - 1) * p.ldb + fq * 16;
+  const uint8_t* Bs = p.Bs + (long)(min(n0 + fr, p.N - 1) >> p.bshift) * p.ldsb;
+  const uint8_t* A[RM];
+  const uint8_t* As[RM];
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    const long m = min(m0 + i * 16 + fr, p.M - 1);
+    A[i] = p.A + m * p.lda + fq * 16;
+    As[i] = p.As + m * p.ldsa;
+  }
+  f32x4 acc[RM];
+#pragma unroll
+  for (int i = 0; i < RM; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int kt = k0; kt < k1; ++kt) {
+    const uint8_t* b = B + (long)kt * 128;
+    const i32x8 wb = frag8((const char*)b, (const char*)b + 64);
+    const int sw = Bs[kt];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const uint8_t* a = A[i] + (long)kt * 128;
+      const i32x8 xa = frag8((const char*)a, (const char*)a + 64);
+      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wb, xa, acc[i], 0, 0, 0, sw, 0, (int)As[i][kt]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) part[wid][i][lane] = acc[i];
+  __syncthreads();
+  if (tid >= RM * 64) return;
+  const int i = wid;  // wave i joins fragment i
+  f32x4 s = part[0][i][lane];
+#pragma unroll
+  for (int w = 1; w < W; ++w) s += part[w][i][lane];
+  float bias[4];
+  bias4(p, n0 + fq * 4, bias);
+  store4<ACT, CT>(p, m0 + i * 16 + fr, n0 + fq * 4, s, bias);
 }
 
 // ---- the large tile ----
@@ -181,15 +290,6 @@ DEVI void mma_step(f32x4& acc, const i32x8& b, const i32x8& a, uint32_t sb, uint
     asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
   else
     asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
-}
-
-DEVI void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, int soff, char* lds_wave_base) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 16, voff, soff, 0, 0);
-}
-
-DEVI i32x8 frag8(const char* lo, const char* hi) {
-  const int4 l = *(const int4*)lo, h = *(const int4*)hi;
-  return (i32x8){l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
 }
 
 constexpr int BIG_STAGE = 512 * 128;
@@ -371,13 +471,37 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
   }
 }
 
+template <int BM, int BN, int S, int ACT, int CT>
+void launch_tile(const Fp8Gemm& p, hipStream_t s) {
+  hipLaunchKernelGGL((fp8_gemm_kernel<BM, BN, 2, 2, S, ACT, CT>), dim3(cdiv(p.M, BM) * cdiv(p.N, BN)), dim3(256), 0, s, p);
+}
+
+template <int RM, int ACT, int CT>
+void launch_few(const Fp8Gemm& p, hipStream_t s) {
+  hipLaunchKernelGGL((fp8_gemm_few_kernel<RM, ACT, CT>), dim3(cdiv(p.N, 16), cdiv(p.M, 16 * RM)), dim3(512), 0, s, p);
+}
+
+int g_force = -1;  // tests and measurements: run this kernel whatever the sizes (fp8_gemm_force)
+
 template <int ACT, int CT>
 void launch(const Fp8Gemm& p, hipStream_t s) {
-  // (32-bit offsets inside a tile: 256 rows of at most 2^22 bytes)
-  if (p.bshift == 7 && p.M >= 512 && p.N >= 512 && p.lda <= (1 << 22) && p.ldb <= (1 << 22))
-    hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3(cdiv(p.M, 256) * cdiv(p.N, 256)), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((fp8_gemm_kernel<128, 128, 2, 2, ACT, CT>), dim3(cdiv(p.M, 128) * cdiv(p.N, 128)), dim3(256), 0, s, p);
+  const long t256 = (long)cdiv(p.M, 256) * cdiv(p.N, 256), t128 = (long)cdiv(p.M, 128) * cdiv(p.N, 128);
+  // (the tiled kernels keep 32-bit offsets inside a tile: 256 rows of at most 2^22 bytes)
+  const bool narrow = p.lda <= (1 << 22) && p.ldb <= (1 << 22);
+  int pick = 0;
+  if (!narrow || p.M <= 64) pick = p.M <= 16 ? 0 : p.M <= 32 ? 1 : 2;
+  else if (p.bshift == 7 && t256 >= 128) pick = 5;
+  else if (t128 >= 128) pick = 4;
+  else pick = 3;
+  if (g_force >= 0 && (g_force < 3 || narrow) && (g_force != 5 || p.bshift == 7)) pick = g_force;
+  switch (pick) {
+    case 0: launch_few<1, ACT, CT>(p, s); break;
+    case 1: launch_few<2, ACT, CT>(p, s); break;
+    case 2: launch_few<4, ACT, CT>(p, s); break;
+    case 3: launch_tile<64, 64, 4, ACT, CT>(p, s); break;
+    case 4: launch_tile<128, 128, 2, ACT, CT>(p, s); break;
+    default: hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3((unsigned)t256), dim3(256), 0, s, p);
+  }
 }
 
 template <int ACT>
@@ -389,11 +513,14 @@ void launch_act(const Fp8Gemm& p, int ctype, hipStream_t s) {
 
 }  // namespace
 
+void fp8_gemm_force(int k) { g_force = k; }
+
 int fp8_gemm_launch(const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, void* C,
                     const float* bias, int M, int N, int nk, long lda, long ldb, int ldsa, int ldsb, int bshift,
                     long ldc, int act, int ctype, hipStream_t s) {
   if (M <= 0 || N <= 0 || nk <= 0) return 0;
   const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, lda, ldb, ldsa, ldsb, bshift, ldc};
+  if (lda > (1 << 22) && cdiv(M, 64) > 65535) return (int)hipErrorInvalidValue;  // (grid of the few-row kernel)
   if (act == ACT_NONE) launch_act<ACT_NONE>(p, ctype, s);
   else if (act == ACT_RELU) launch_act<ACT_RELU>(p, ctype, s);
   else launch_act<ACT_SILU>(p, ctype, s);

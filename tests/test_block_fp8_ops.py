@@ -548,6 +548,23 @@ def test_matmul_fp8_integers_are_exact(dev, m, n, k, tile):
     assert torch.equal(got.double().cpu(), (ref + bias.double()).clamp(min=0))
 
 
+@gpu
+@pytest.mark.parametrize("kernel", range(6))
+@pytest.mark.parametrize("m,n,k", [(1, 16, 128), (5, 100, 130), (70, 130, 1000), (150, 260, 1281), (300, 515, 640), (257, 129, 2176)])
+def test_matmul_fp8_every_kernel(kernel, m, n, k):
+    """Each kernel at sizes that the choice by size would give to another: exact on integers, every output type."""
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    keep = hip.C.fp8_gemm_force
+    keep(kernel)
+    try:
+        for tile in (1, 128):
+            test_matmul_fp8_integers_are_exact("cuda", m, n, k, tile)
+        for t, act in ((torch.bfloat16, "silu"), (torch.float16, "relu"), (torch.float32, None)):
+            test_matmul_fp8("cuda", t, m, n, k, act)
+    finally:
+        keep(-1)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("m,n,k,act", [(1, 130, 256, "silu"), (33, 64, 2048, "relu"), (129, 257, 1000, None), (300, 300, 896, "silu"),
