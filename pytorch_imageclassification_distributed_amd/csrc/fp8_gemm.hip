@@ -267,60 +267,54 @@ __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
 }
 
 // ---- the large tile ----
-// 256 x 256 on 4 waves of 128 x 128, one block a CU.  A k-step of a wave is 64 MFMAs fed by 32 ds_read_b128: (128 + 128)
-// rows x 128 B x 4 waves + the 64 KB that LDS-DMA writes are 192 KB a step through the LDS port, against 256 KB for
-// 8 waves of 128 x 64 (where the port, not the matrix pipe, would set the pace).  The 256 accumulators of a lane live in
-// AGPRs, the fragments of one k-step in 128 VGPRs; the step runs in two halves of four B fragments each (all eight A
-// fragments in both), so that every register is refilled where its last MFMA has been issued:
-//   first half of step kt (B 0-3):   B 4-7 of kt are read;
+// 256 x 256 on 4 waves of 128 x 128, one block a CU.  A k-step of a wave is 32 MFMAs of 32 x 32 x 64 fed by 32
+// ds_read_b128: (128 + 128) rows x 128 B x 4 waves + the 64 KB that LDS-DMA writes are 192 KB a step through the LDS
+// port, against 256 KB for 8 waves of 128 x 64 (where the port, not the matrix pipe, would set the pace).  The 256
+// accumulators of a lane live in AGPRs, the fragments of one k-step in 128 VGPRs; the step runs in two halves of two B
+// blocks each (all four A blocks in both), so that every register is refilled where its last MFMA has been issued:
+//   first half of step kt (B 0, 1):  B 2, 3 of kt are read;
 //   middle: tile kt + 1 has landed, this buffer's reads have ended in every wave: the step's one barrier;
-//   second half (B 4-7):             the 16 LDS-DMA pieces of tile kt + 2 go into this buffer, and B 0-3 and, row by
-//                                    row, A of kt + 1 are read from the other one.
-// One memory instruction or two stand between two MFMAs; a tile has a whole step (64 x 32 cycles) to arrive.
-// The MFMAs are asm statements (accumulators pinned to AGPRs, order kept); each carries the two wait states between a
-// VALU write and a matrix read.
+//   second half (B 2, 3):            the 16 LDS-DMA pieces of tile kt + 2 go into this buffer, one an MFMA (two an MFMA
+//                                    stall at the 64 B a cycle of the load path: 206 us against 186), and B 0, 1 and,
+//                                    block by block, A of kt + 1 are read from the other one.
+// 8192 x 8192 x 4096: 211 us (2.6 PFLOP/s), 186 of it the main loop; with loads that always hit L2, or a prefetch into
+// L2, no faster; without any load 170 (the clock under full load), so the matrix pipe bounds it.  The rest is the
+// epilogue and a block's first loads; persistent blocks that issue the next tile's loads before the outputs were slower
+// (249 us: their registers spill).
+// The MFMAs are asm statements (accumulators pinned to AGPRs, order kept).  hipcc knows nothing of their hazards: their
+// operands come from LDS (its waits see asm operands), a VALU result (the scales) passes a wait of its own, an
+// accumulator is used again two MFMAs (128 cycles) later, and the epilogue reads them behind a wait that depends on all of them.
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
 template <int R>
-DEVI void mma_step(f32x4& acc, const i32x8& b, const i32x8& a, uint32_t sb, uint32_t sa) {
-  static_assert(R >= 0 && R < 4, "scale byte");
+DEVI void mma32(f32x16_t& acc, const i32x8& b, const i32x8& a, uint32_t sb, uint32_t sa) {
+  static_assert(R == 0 || R == 1, "scale byte");
   if constexpr (R == 0)
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
-  else if constexpr (R == 1)
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
-  else if constexpr (R == 2)
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
   else
-    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
+    asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[1,1,0] op_sel_hi:[0,0,0]" : "+a"(acc) : "v"(b), "v"(a), "v"(sb), "v"(sa) : "memory");
 }
 
 constexpr int BIG_STAGE = 512 * 128;
-constexpr int BIG_CST = 256 + 8;  // 16-bit elements a row of the staged output tile: 4 rows differ by 16 banks
-constexpr int BIG_BUF = 128 * BIG_CST * 2 > BIG_STAGE ? 128 * BIG_CST * 2 : BIG_STAGE;  // half of the output tile each
+constexpr int BIG_BAND = 4;     // tile rows of a band
 
 template <int ACT, int CT>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
-  // two arrays, not one: hipcc makes an LDS read wait for every LDS-DMA that may write what it reads, and tells them
-  // apart by the array alone
-  __shared__ __attribute__((aligned(16))) char buf0[BIG_BUF];
-  __shared__ __attribute__((aligned(16))) char buf1[BIG_BUF];
+  // separate arrays, not one: hipcc makes an LDS read wait for every LDS-DMA that may write what it reads, and tells
+  // them apart by the array alone
+  __shared__ __attribute__((aligned(16))) char buf0[BIG_STAGE];
+  __shared__ __attribute__((aligned(16))) char buf1[BIG_STAGE];
+  __shared__ __attribute__((aligned(16))) char out[4][32 * 256];  // a wave's 32 x 128 16-bit outputs
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wid >> 1, wn = wid & 1;
   const int gm = (p.M + 255) >> 8, gn = (p.N + 255) >> 8;
-  const int lin = xcd_remap(blockIdx.x, gm * gn);
-  // an XCD's consecutive tiles walk a band of 4 tile rows column by column: its L2 then holds 4 row panels and a few
-  // column panels at a time
-  const int band = lin / (4 * gn), first = band * 4, rows = min(gm - first, 4), rest = lin - band * 4 * gn;
-  const int m0 = __builtin_amdgcn_readfirstlane((first + rest % rows) * 256);
-  const int n0 = __builtin_amdgcn_readfirstlane((rest / rows) * 256);
+  const int lda = (int)p.lda, ldb = (int)p.ldb, nk = p.nk;
 
   // LDS-DMA sources: piece q of a wave is rows [64 wid + 8 q, + 8) of its 256; lane l brings 16-B chunk (l & 7) of row
   // l >> 3, from source chunk (l & 7) ^ ((row >> 1) & 7), which takes two values over q.  Rows past the end are past
   // the buffer resource: zeros.
   const int lrow = lane >> 3, pch = lane & 7;
-  const long abytes = (long)(p.M - m0) * p.lda, bbytes = (long)(p.N - n0) * p.ldb;
-  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.A + (long)m0 * p.lda, abytes), rb = make_rsrc(p.B + (long)n0 * p.ldb, bbytes);
-  const __amdgpu_buffer_rsrc_t za = make_rsrc(p.A, 0);
-  const int lda = (int)p.lda, ldb = (int)p.ldb;
   unsigned va[2], vb[2];
 #pragma unroll
   for (int o = 0; o < 2; ++o) {
@@ -328,41 +322,88 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
     va[o] = (unsigned)((wid * 64 + lrow) * lda + ch);
     vb[o] = (unsigned)((wid * 64 + lrow) * ldb + ch);
   }
+  const int fr = lane & 31, fh = lane >> 5;
+  // fragment (block i, half s) of a buffer: row 32 i + fr of the wave's 128, chunks 4 s + fh and 4 s + fh + 2 (the
+  // swizzle depends on fr alone)
+  int oa[4], ob[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    oa[c] = swz(wm * 128 + fr, 2 * c + fh);  // chunk 2 c + fh
+    ob[c] = 256 * 128 + swz(wn * 128 + fr, 2 * c + fh);
+  }
+  auto frag = [&](const char* buf, const int* o, int i, int s) __attribute__((always_inline)) {
+    return frag8(buf + o[2 * s] + i * 4096, buf + o[2 * s + 1] + i * 4096);
+  };
+
+  // an XCD's consecutive tiles walk a band of tile rows column by column, so that its L2 holds four row panels and a few
+  // column panels at a time
+  const int lin = xcd_remap(blockIdx.x, gm * gn);
+  const int band = lin / (BIG_BAND * gn), first = band * BIG_BAND, rows = min(gm - first, BIG_BAND);
+  const int rest = lin - band * BIG_BAND * gn;
+  const int m0 = __builtin_amdgcn_readfirstlane((first + rest % rows) * 256);
+  const int n0 = __builtin_amdgcn_readfirstlane(rest / rows * 256);
+  const __amdgpu_buffer_rsrc_t za = make_rsrc(p.A, 0);
+  const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.A + (long)m0 * p.lda, (long)(p.M - m0) * p.lda);
+  const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.B + (long)n0 * p.ldb, (long)(p.N - n0) * p.ldb);
+  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(p.As + (long)m0 * p.ldsa, (long)(p.M - m0) * p.ldsa);
+  const uint32_t* wsb = (const uint32_t*)(p.Bs + (long)(min(n0 + wn * 128, p.N - 1) >> 7) * p.ldsb);
   auto piece = [&](int kt, char* buf, int q, bool live) __attribute__((always_inline)) {
     char* dst = buf + (wid * 64 + (q & 7) * 8) * 128;
     if (q < 8) dma16(live ? ra : za, va[q & 1], kt * 128 + q * 8 * lda, dst);
     else dma16(live ? rb : za, vb[q & 1], kt * 128 + (q - 8) * 8 * ldb, dst + 256 * 128);
   };
-
-  const int fr = lane & 15, fq = lane >> 4;
-  // fragment i of a buffer: row 16 i + fr of the wave's 128, chunks fq and fq + 4 (the swizzle depends on fr alone)
-  const int oa = swz(wm * 128 + fr, fq), oah = swz(wm * 128 + fr, fq + 4);
-  const int ob = 256 * 128 + swz(wn * 128 + fr, fq), obh = 256 * 128 + swz(wn * 128 + fr, fq + 4);
-
   // scales: a word holds four k-steps' bytes; a pair of steps takes bytes 0 and 1, then the words are shifted.  The next
   // words are loaded four steps ahead.  An odd number of steps runs one more on zeros (the DMA pieces past the end come
   // from an empty resource); its scale byte is cleared, so that padding cannot hold a NaN scale.
-  const int nk = p.nk;
-  const __amdgpu_buffer_rsrc_t rsa = make_rsrc(p.As + (long)m0 * p.ldsa, (long)(p.M - m0) * p.ldsa);
   const int vsa = (wm * 128 + fr) * p.ldsa;
-  const uint32_t* wsb = (const uint32_t*)(p.Bs + (long)(min(n0 + wn * 128, p.N - 1) >> 7) * p.ldsb);
   const int words = (nk + 3) >> 2;
   const uint32_t last = (nk & 3) ? (1u << (8 * (nk & 3))) - 1 : ~0u;
-  uint32_t sx[8], nx[8], sw, nw;
+  uint32_t sx[4], nx[4], sw, nw;
   auto scales = [&](int word) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) nx[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa, word * 4 + i * 16 * p.ldsa, 0);
+    for (int i = 0; i < 4; ++i) nx[i] = __builtin_amdgcn_raw_buffer_load_b32(rsa, vsa, word * 4 + i * 32 * p.ldsa, 0);
     nw = wsb[word];
   };
+  // the words have arrived (called behind a wait that covers them): without this hipcc waits again, for everything, where
+  // they are used
+  auto scales_here = [&]() __attribute__((always_inline)) {
+    asm volatile("" : "+v"(nx[0]), "+v"(nx[1]), "+v"(nx[2]), "+v"(nx[3]), "+v"(nw));
+  };
 
-  f32x4 acc[8][8];
+  f32x16_t acc[4][4];
+  i32x8 a[4][2], b[4][2];
+  auto step = [&](auto rc, int kt) __attribute__((always_inline)) {
+    constexpr int P = decltype(rc)::value;  // kt & 1
+    auto cur = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf0; else return (char*)buf1; };
+    auto nxt = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf1; else return (char*)buf0; };
+    // MFMA t of a half: A block t / 4, k-half (t >> 1) & 1, B block t & 1 of the half's two
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+    for (int t = 0; t < 16; ++t) {
+      const int i = t >> 2, s = (t >> 1) & 1, j = t & 1;
+      mma32<P>(acc[i][j], b[j][s], a[i][s], sw, sx[i]);
+      if (t < 8 && (t & 1) == 0) b[2 + (t >> 2)][(t >> 1) & 1] = frag(cur(), ob, 2 + (t >> 2), (t >> 1) & 1);
+    }
+    wait_vmcnt<0>();
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    if constexpr (P == 0) {
+      if ((kt & 2) == 0) scales(min((kt >> 2) + 1, words - 1));
+    } else {
+      scales_here();
+    }
+    const bool live = kt + 2 < nk;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  asm volatile("s_nop 7");
+    for (int t = 0; t < 16; ++t) {
+      const int i = t >> 2, s = (t >> 1) & 1, j = 2 + (t & 1);
+      mma32<P>(acc[i][j], b[j][s], a[i][s], sw, sx[i]);
+      piece(kt + 2, cur(), t, live);
+      if (t >= 2 && t < 10 && (t & 1) == 0) b[(t - 2) >> 2][((t - 2) >> 1) & 1] = frag(nxt(), ob, (t - 2) >> 2, ((t - 2) >> 1) & 1);
+      if ((t & 3) == 1) a[i][0] = frag(nxt(), oa, i, 0);
+      if ((t & 3) == 3) a[i][1] = frag(nxt(), oa, i, 1);
+    }
+  };
 
-  i32x8 a[8], b[8];
+  // the first two k-steps
 #pragma unroll
   for (int q = 0; q < 16; ++q) piece(0, buf0, q, true);
 #pragma unroll
@@ -371,102 +412,100 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
   wait_vmcnt<0>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = frag8(buf0 + oa + i * 2048, buf0 + oah + i * 2048);
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = frag8(buf0 + ob + j * 2048, buf0 + obh + j * 2048);
-
-  auto step = [&](auto rc, int kt) __attribute__((always_inline)) {
-    constexpr int P = decltype(rc)::value;  // kt & 1
-    auto cur = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf0; else return (char*)buf1; };
-    auto nxt = [&]() __attribute__((always_inline)) { if constexpr (P == 0) return (char*)buf1; else return (char*)buf0; };
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x16_t{};
+  asm volatile("s_nop 7");
 #pragma unroll
-    for (int t = 0; t < 32; ++t) {
-      const int i = t >> 2, j = t & 3;
-      mma_step<P>(acc[i][j], b[j], a[i], sw, sx[i]);
-      if ((t & 3) == 1 && t < 16) b[4 + (t >> 2)] = frag8(cur() + ob + (4 + (t >> 2)) * 2048, cur() + obh + (4 + (t >> 2)) * 2048);
-    }
-    wait_vmcnt<0>();
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    const bool live = kt + 2 < nk;
+  for (int i = 0; i < 4; ++i) {
+    a[i][0] = frag(buf0, oa, i, 0);
+    a[i][1] = frag(buf0, oa, i, 1);
+  }
 #pragma unroll
-    for (int t = 0; t < 32; ++t) {
-      const int i = t >> 2, j = 4 + (t & 3);
-      mma_step<P>(acc[i][j], b[j], a[i], sw, sx[i]);
-      if (t < 16) piece(kt + 2, cur(), t, live);
-      if ((t & 3) == 2 && t < 16) b[t >> 2] = frag8(nxt() + ob + (t >> 2) * 2048, nxt() + obh + (t >> 2) * 2048);
-      if (j == 7) a[i] = frag8(nxt() + oa + i * 2048, nxt() + oah + i * 2048);
-    }
-  };
-  for (int kt = 0; kt < nk; kt += 2) {
+  for (int j = 0; j < 2; ++j) {
+    b[j][0] = frag(buf0, ob, j, 0);
+    b[j][1] = frag(buf0, ob, j, 1);
+  }
+  scales_here();
+  int kt = 0;
+  do {
     if ((kt & 2) == 0) {
       const uint32_t m = (kt >> 2) == words - 1 ? last : ~0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sx[i] = nx[i] & m;
+      for (int i = 0; i < 4; ++i) sx[i] = nx[i] & m;
       sw = nw & m;
-      scales(min((kt >> 2) + 1, words - 1));
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sx[i] >>= 16;
+      for (int i = 0; i < 4; ++i) sx[i] >>= 16;
       sw >>= 16;
     }
+    asm volatile("s_nop 1" : "+v"(sx[0]), "+v"(sx[1]), "+v"(sx[2]), "+v"(sx[3]), "+v"(sw));  // VALU result -> MFMA
     step(std::integral_constant<int, 0>{}, kt);
     step(std::integral_constant<int, 1>{}, kt + 1);
-  }
-  wait_vmcnt<0>();
+    kt += 2;
+  } while (kt < nk);
   // the last MFMAs' results before the first read of an accumulator: waits that every accumulator depends on
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]), "+a"(acc[i][4]), "+a"(acc[i][5]), "+a"(acc[i][6]), "+a"(acc[i][7]));
-  __syncthreads();
-  float bias[8][4];
+  for (int i = 0; i < 4; ++i)
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]));
+  wait_vmcnt<0>();  // (LDS-DMA must not outlive the block)
+  const int cm = m0 + wm * 128, cn = n0 + wn * 128;
+  const bool whole = m0 + 256 <= p.M && n0 + 256 <= p.N && (p.ldc & 7) == 0;
+  // bias: past N (and without one) the resource gives zeros
+  const __amdgpu_buffer_rsrc_t rbias = make_rsrc(p.bias, p.bias != nullptr ? (long)p.N * 4 : 0);
+  float bias[4][4][4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = n0 + wn * 128 + j * 16 + fq * 4 + r;
-      bias[j][r] = p.bias != nullptr && n < p.N ? p.bias[n] : 0.f;
-    }
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        bias[j][g][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rbias, (cn + fh * 4) * 4, (j * 32 + g * 8 + r) * 4, 0));
+  // acc[i][j][4 g + r]: row 32 i + fr, column 32 j + 8 g + 4 fh + r of the wave's 128 x 128
   if constexpr (CT == C_F32) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int m = m0 + wm * 128 + i * 16 + fr;
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int n = n0 + wn * 128 + j * 16 + fq * 4 + r;
-          if (m < p.M && n < p.N) store_c<CT>(p, (long)m * p.ldc + n, apply_act(acc[i][j][r] + bias[j][r], ACT));
-        }
+        for (int g = 0; g < 4; ++g)
+          store4<ACT, CT>(p, cm + i * 32 + fr, cn + j * 32 + g * 8 + fh * 4,
+                          (f32x4){acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]},
+                          bias[j][g]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    return;
-  }
-  // 16-bit outputs go through LDS, so that rows leave in whole 16-B chunks of 512 contiguous bytes
-  uint16_t* ct = (uint16_t*)(wm == 0 ? buf0 : buf1);  // rows 0-127 and 128-255 of the tile
+  } else {
+    // 16-bit outputs pass through the wave's own LDS, 32 rows at a time, and leave in 16-B chunks, 256 contiguous bytes
+    // a row.  16-B chunk c of row r sits at c ^ (r & 15): neither side meets a bank conflict.
+    char* st = out[wid];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float v[4];
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = apply_act(acc[i][j][r] + bias[j][r], ACT);
-      *(uint2*)(ct + (i * 16 + fr) * BIG_CST + wn * 128 + j * 16 + fq * 4) = make_uint2(pack_c<CT>(v[0], v[1]), pack_c<CT>(v[2], v[3]));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  }
-  __syncthreads();
-  uint16_t* C = (uint16_t*)p.C;
-  const int cc = (tid & 31) * 8;
-  const int nv = min(8, p.N - n0 - cc);
-  const bool vec = (p.ldc & 7) == 0;
-  for (int r = tid >> 5; r < 256 && m0 + r < p.M; r += 8) {
-    const uint4 v = *(const uint4*)((const uint16_t*)(r < 128 ? buf0 : buf1) + (r & 127) * BIG_CST + cc);
-    uint16_t* o = C + (long)(m0 + r) * p.ldc + n0 + cc;
-    if (vec && nv == 8) *(uint4*)o = v;
-    else {
-      const uint16_t* e = (const uint16_t*)&v;
-      for (int k = 0; k < nv; ++k) o[k] = e[k];
+        for (int g = 0; g < 4; ++g) {
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = apply_act(acc[i][j][4 * g + r] + bias[j][g][r], ACT);
+          *(uint2*)(st + fr * 256 + (((j * 4 + g) ^ (fr & 15)) << 4) + fh * 8) = make_uint2(pack_c<CT>(v[0], v[1]), pack_c<CT>(v[2], v[3]));
+          if (g == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+      const int c = lane & 15, r0 = lane >> 4;
+      uint16_t* C = (uint16_t*)p.C + (long)(cm + i * 32 + r0) * p.ldc + cn + c * 8;
+      if (whole) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *(uint4*)(C + (long)q * 4 * p.ldc) = *(const uint4*)(st + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
+      } else {
+        const int nv = min(8, p.N - cn - c * 8);
+#pragma unroll 1
+        for (int q = 0; q < 8 && cm + i * 32 + q * 4 + r0 < p.M; ++q) {
+          const uint16_t* e = (const uint16_t*)(st + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
+#pragma unroll 1
+          for (int k = 0; k < nv; ++k) C[(long)q * 4 * p.ldc + k] = e[k];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
@@ -483,24 +522,52 @@ void launch_few(const Fp8Gemm& p, hipStream_t s) {
 
 int g_force = -1;  // tests and measurements: run this kernel whatever the sizes (fp8_gemm_force)
 
+// Which kernel: the one whose time this estimates lowest, in us, from what each measured on 256 CUs - a round of blocks
+// costs so much a k-step, plus its first loads and its outputs.  Measured (K 4096 unless given; kernel: us):
+//   16 x 4096        few16 7.0   64x64 10.2   128x64 -     128x128(4) -     128x128(2) 29   256 46
+//   32 x 4096        few32 9.6   64x64 10.6
+//   64 x 4096        few32 16.6  64x64 11.2
+//   512 x 4096                   64x64 23.0   128x64 18.2  128x128(4) 24.1  128x128(2) 34   256 41
+//   1024 x 4096                  64x64 42.8   128x64 33.9  128x128(4) 28.4  128x128(2) 36   256 41
+//   2048 x 4096                  64x64 82.7   128x64 73.5  128x128(4) 59.0  128x128(2) 50   256 57
+//   4096 x 4096                  64x64 161    128x64 146   128x128(4) 117   128x128(2) 98   256 65
+//   8192 x 2048, K 512           64x64 37.5   128x64 41.9  128x128(4) 34.5  128x128(2) 26   256 19
+enum { K_FEW16, K_FEW32, K_64, K_128x64, K_128_4, K_128_2, K_256, K_COUNT };
+
+double estimate(int k, const Fp8Gemm& p) {
+  auto rounds = [&](int bm, int bn, int slots) { return (double)(((long)cdiv(p.M, bm) * cdiv(p.N, bn) + slots - 1) / slots); };
+  const long t64 = (long)cdiv(p.M, 64) * cdiv(p.N, 64);
+  switch (k) {
+    case K_FEW16: return 2.5 + 0.0005 * cdiv(p.N, 16) * cdiv(p.M, 16) * p.nk;
+    case K_FEW32: return 2.5 + 0.00077 * cdiv(p.N, 16) * cdiv(p.M, 32) * p.nk;
+    case K_64: return rounds(64, 64, 512) * ((t64 <= 256 ? 0.40 : 0.66) * p.nk + 2);  // two blocks a CU
+    case K_128x64: return rounds(128, 64, 256) * (0.50 * p.nk + 2.5);
+    case K_128_4: return rounds(128, 128, 256) * (0.74 * p.nk + 4);
+    case K_128_2: return rounds(128, 128, 512) * (1.05 * p.nk + 7);  // two blocks a CU
+    default: return rounds(256, 256, 256) * (1.05 * p.nk + 11);
+  }
+}
+
 template <int ACT, int CT>
 void launch(const Fp8Gemm& p, hipStream_t s) {
-  const long t256 = (long)cdiv(p.M, 256) * cdiv(p.N, 256), t128 = (long)cdiv(p.M, 128) * cdiv(p.N, 128);
-  // (the tiled kernels keep 32-bit offsets inside a tile: 256 rows of at most 2^22 bytes)
-  const bool narrow = p.lda <= (1 << 22) && p.ldb <= (1 << 22);
-  int pick = 0;
-  if (!narrow || p.M <= 64) pick = p.M <= 16 ? 0 : p.M <= 32 ? 1 : 2;
-  else if (p.bshift == 7 && t256 >= 128) pick = 5;
-  else if (t128 >= 128) pick = 4;
-  else pick = 3;
-  if (g_force >= 0 && (g_force < 3 || narrow) && (g_force != 5 || p.bshift == 7)) pick = g_force;
+  auto fits = [&](int k) {
+    if (k <= K_FEW32) return cdiv(p.M, 16) <= 65535;              // grid.y
+    if (p.lda > (1 << 22) || p.ldb > (1 << 22)) return false;     // 32-bit offsets inside a tile of 256 rows
+    return k != K_256 || p.bshift == 7;                           // it takes one scale for its 128 columns
+  };
+  int pick = K_FEW32;
+  double best = 1e30;
+  for (int k = 0; k < K_COUNT; ++k)
+    if (fits(k) && estimate(k, p) < best) best = estimate(pick = k, p);
+  if (g_force >= 0 && g_force < K_COUNT && fits(g_force)) pick = g_force;
   switch (pick) {
-    case 0: launch_few<1, ACT, CT>(p, s); break;
-    case 1: launch_few<2, ACT, CT>(p, s); break;
-    case 2: launch_few<4, ACT, CT>(p, s); break;
-    case 3: launch_tile<64, 64, 4, ACT, CT>(p, s); break;
-    case 4: launch_tile<128, 128, 2, ACT, CT>(p, s); break;
-    default: hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3((unsigned)t256), dim3(256), 0, s, p);
+    case K_FEW16: launch_few<1, ACT, CT>(p, s); break;
+    case K_FEW32: launch_few<2, ACT, CT>(p, s); break;
+    case K_64: launch_tile<64, 64, 4, ACT, CT>(p, s); break;
+    case K_128x64: launch_tile<128, 64, 4, ACT, CT>(p, s); break;
+    case K_128_4: launch_tile<128, 128, 4, ACT, CT>(p, s); break;
+    case K_128_2: launch_tile<128, 128, 2, ACT, CT>(p, s); break;
+    default: hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3((unsigned)(cdiv(p.M, 256) * cdiv(p.N, 256))), dim3(256), 0, s, p);
   }
 }
 
@@ -520,7 +587,7 @@ int fp8_gemm_launch(const uint8_t* A, const uint8_t* As, const uint8_t* B, const
                     long ldc, int act, int ctype, hipStream_t s) {
   if (M <= 0 || N <= 0 || nk <= 0) return 0;
   const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, lda, ldb, ldsa, ldsb, bshift, ldc};
-  if (lda > (1 << 22) && cdiv(M, 64) > 65535) return (int)hipErrorInvalidValue;  // (grid of the few-row kernel)
+  if (lda > (1 << 22) && cdiv(M, 16) > 65535) return (int)hipErrorInvalidValue;  // (grid of the few-row kernels)
   if (act == ACT_NONE) launch_act<ACT_NONE>(p, ctype, s);
   else if (act == ACT_RELU) launch_act<ACT_RELU>(p, ctype, s);
   else launch_act<ACT_SILU>(p, ctype, s);

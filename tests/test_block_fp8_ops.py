@@ -549,7 +549,7 @@ def test_matmul_fp8_integers_are_exact(dev, m, n, k, tile):
 
 
 @gpu
-@pytest.mark.parametrize("kernel", range(6))
+@pytest.mark.parametrize("kernel", range(7))
 @pytest.mark.parametrize("m,n,k", [(1, 16, 128), (5, 100, 130), (70, 130, 1000), (150, 260, 1281), (300, 515, 640), (257, 129, 2176)])
 def test_matmul_fp8_every_kernel(kernel, m, n, k):
     """Each kernel at sizes that the choice by size would give to another: exact on integers, every output type."""
