@@ -1081,13 +1081,6 @@ class PeerComm {
 
 }  // namespace
 
-// (block_bindings.cpp) the weight gradient of a dense layer: a 1x1 convolution over 1x1 maps
-void dense_wgrad(Tensor dY, Tensor X, Tensor dW, int M, int Cout, int Cin, int k_per_split, int splits, Tensor zero,
-                 int stages, OT ws) {
-  conv_wgrad(dY, X, dW, M, Cout, Cin, Cin, 1, 1, 1, 1, 1, 1, 0, 0, 1, 1, 1, k_per_split, splits, zero, stages, ws, 0, OT(),
-             OT(), OT(), 0);
-}
-
 void register_loader(pybind11::module& m);  // loader.cpp: native image-folder loader
 void register_block_ops(pybind11::module& m);  // block_bindings.cpp: dropout / RMS norm / 8-bit linear block
 void bn_set_reduce_blocks(int n, int chb);

@@ -32,11 +32,9 @@ int quant_rows_launch(const void*, const void*, uint8_t*, uint8_t*, bf16_t*, flo
 int quant_tiles_launch(const void*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, int, int, long, int, long, int, int,
                        hipStream_t);
 int dequant_launch(const uint8_t*, const uint8_t*, void*, long, int, long, int, int, int, hipStream_t);
-int zero_f32_launch(float*, long, hipStream_t);
+int rows_grad_splits(int, int, int, int);
+int rows_grad_launch(const bf16_t*, const bf16_t*, float*, float*, int, int, int, int, int, int, hipStream_t);
 void fp8_gemm_force(int);
-// bindings.cpp: dW[Cout][Cin] += dY[M][Cout]^T X[M][Cin], bf16, Cout and Cin multiples of 8
-void dense_wgrad(Tensor dY, Tensor X, Tensor dW, int M, int Cout, int Cin, int k_per_split, int splits, Tensor zero,
-                 int stages, std::optional<Tensor> ws);
 int fp8_gemm_launch(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, const float*, int, int, int,
                     long, long, int, int, int, long, int, int, hipStream_t);
 
@@ -455,27 +453,23 @@ Tensor op_matmul(const Tensor& a, const Tensor& as, const Tensor& b, const Tenso
   return c;
 }
 
-// dw[n][k] = sum over the m rows of dy[row][n] x[row][k] on the bf16 weight-gradient kernels (the rows are the pixels of
-// a 1x1 convolution over 1x1 maps).  dy, x: widths rounded up to 8.
-void rows_grad(const Tensor& dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k, const Tensor& zero) {
+// dw[n][k] = sum over the m rows of dy[row][n] x[row][k]; dy, x: bf16, widths n, k rounded up to 8
+void rows_grad(const Tensor& dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k) {
   const c10::DeviceGuard guard(dw.device());
-  const int64_t n8 = (n + 7) / 8 * 8, k8 = (k + 7) / 8 * 8;
-  const bool direct = n8 == n && k8 == k;
-  const Tensor out = direct ? dw : fresh({n8, k8}, dw, at::kFloat);
-  ok(zero_f32_launch(out.data_ptr<float>(), out.numel(), stream_of(out)), "zero");
-  if (m > 0) {
-    const int stages = n8 >= 256 && k8 >= 256 ? 7 : 2;
-    const int64_t side = stages == 7 ? 256 : 128;
-    const int64_t rows = n8 > 64 ? side : 64, tiles = ((n8 + rows - 1) / rows) * ((k8 + side - 1) / side);
-    // at most 8 slabs: they are added in one ordered pass
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({8, 512 / tiles, m / 512}));
-    const int64_t kps = ((m + splits - 1) / splits + 63) / 64 * 64;
-    splits = (m + kps - 1) / kps;
-    OT slabs;
-    if (splits > 1) slabs = fresh({splits * n8 * k8}, dw, at::kFloat);
-    dense_wgrad(dy, x, out, (int)m, (int)n8, (int)k8, (int)kps, (int)splits, zero, stages, slabs);
-  }
-  if (!direct) dw.copy_(out.narrow(0, 0, n).narrow(1, 0, k));
+  const int64_t ldy = (n + 7) / 8 * 8, ldx = (k + 7) / 8 * 8;
+  typed(dy, dw, at::kBFloat16, m * ldy, "dy");
+  typed(x, dw, at::kBFloat16, m * ldx, "x");
+  TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.is_contiguous() && dw.numel() == n * k && ((uintptr_t)dw.data_ptr() & 15) == 0,
+              "linear_fp8: weight gradient must be contiguous float32");
+  TORCH_CHECK(m < (1LL << 31) - 128, "linear_fp8: too many rows");
+  const int splits = rows_grad_splits((int)m, (int)n, (int)k, (int)std::max(ldy, ldx));
+  TORCH_CHECK(splits > 0, "linear_fp8: rows too wide for the weight gradient");
+  Tensor slabs;
+  if (splits > 1) slabs = fresh({splits * n * k}, dw, at::kFloat);
+  ok(rows_grad_launch((const bf16_t*)dy.data_ptr(), (const bf16_t*)x.data_ptr(), dw.data_ptr<float>(),
+                      splits > 1 ? slabs.data_ptr<float>() : nullptr, (int)m, (int)n, (int)k, (int)ldy, (int)ldx, splits,
+                      stream_of(dw)),
+     "linear_fp8 weight gradient");
 }
 
 // y = act(q(x) q(w)^T + b).  Backward: dx = q(dy) q(w) in 8 bits (the weights' transpose was written beside them; 128 x
@@ -509,11 +503,11 @@ LinearOut linear_forward(const Tensor& x, const Tensor& weight, const OT& bias, 
 }
 
 struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weight, const OT& bias, const Tensor& zero,
-                        int64_t act, bool need_x, bool need_w, c10::IValue wslot, c10::IValue bslot) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x_, const Tensor& weight, const OT& bias, int64_t act,
+                        bool need_x, bool need_w, c10::IValue wslot, c10::IValue bslot) {
     const Tensor x = dense16(x_);
     LinearOut o = linear_forward(x, weight, bias, act, need_x, need_w);
-    ctx->save_for_backward({o.xb, o.wt, o.wtsc, act ? o.y : Tensor(), zero});
+    ctx->save_for_backward({o.xb, o.wt, o.wtsc, act ? o.y : Tensor()});
     ctx->saved_data["m"] = x.size(0);
     ctx->saved_data["n"] = weight.size(0);
     ctx->saved_data["k"] = x.size(1);
@@ -551,7 +545,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
     }
     if (nw) {
       dw = slot_or_empty(ctx->saved_data["wslot"], {n, k}, dy);
-      rows_grad(dyb, xb, dw, m, n, k, s[4]);
+      rows_grad(dyb, xb, dw, m, n, k);
       const auto t = (at::ScalarType)ctx->saved_data["wtype"].toInt();
       if (t != at::kFloat) dw = dw.to(t);
     }
@@ -562,15 +556,15 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
       if (t != at::kFloat) db = db.to(t);
     }
     variable_list out = no_second({dx, dw, db});
-    return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
-Tensor op_linear_fp8(const Tensor& x, const Tensor& weight, const OT& bias, const Tensor& zero, int64_t act,
-                     py::object wslot, py::object bslot) {
+Tensor op_linear_fp8(const Tensor& x, const Tensor& weight, const OT& bias, int64_t act, py::object wslot,
+                     py::object bslot) {
   const bool grad = at::GradMode::is_enabled(), nx = grad && x.requires_grad(), nw = grad && weight.requires_grad();
   if (!(nx || nw || (grad && wants(bias)))) return linear_forward(dense16(x.detach()), weight, bias, act, false, false).y;
-  return LinearFp8Node::apply(x, weight, bias, zero, act, nx, nw, slot_value(wslot), slot_value(bslot));
+  return LinearFp8Node::apply(x, weight, bias, act, nx, nw, slot_value(wslot), slot_value(bslot));
 }
 
 }  // namespace

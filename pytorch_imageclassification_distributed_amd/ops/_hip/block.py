@@ -1,7 +1,7 @@
 """Counter-based dropout, root-mean-square norm with the residual's addition and 8-bit linear layers (HIP kernels
-``csrc/block_ops.hip``, ``csrc/fp8_gemm.hip``; autograd nodes and allocation in ``csrc/block_bindings.cpp``).
+``csrc/block_ops.hip``, ``csrc/fp8_gemm.hip``, ``csrc/rows_grad.hip``; autograd nodes and allocation in ``csrc/block_bindings.cpp``).
 
-No kernel here adds with atomics whose order shows, no workspace outlives its call and nothing is read back on the host,
+No kernel here adds with atomics, no workspace outlives its call and nothing is read back on the host,
 so calls may run on any stream, at once, and inside a captured graph.
 """
 from __future__ import annotations
@@ -12,7 +12,7 @@ import torch
 
 from ..fp8_blocks import BLOCK, Fp8Blocks
 from ..grad_arena import grad_buffer
-from .common import ACT, C, ws
+from .common import ACT, C
 
 
 def _drop_state(dev, seed, offset):
@@ -69,7 +69,7 @@ def matmul_fp8(a, b, bias, act, out_dtype):
 
 
 def linear_fp8(x2, weight, bias, act):
-    return C.linear_fp8(x2, weight, bias, ws(x2.device).zero, ACT[act], _slot(weight), _slot(bias))
+    return C.linear_fp8(x2, weight, bias, ACT[act], _slot(weight), _slot(bias))
 
 
 # names this part owns (ops/hip.py re-exports them)
