@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
     asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]));
   wait_vmcnt<0>();  // (LDS-DMA must not outlive the block)
   const int cm = m0 + wm * 128, cn = n0 + wn * 128;
-  const bool whole = m0 + 256 <= p.M && n0 + 256 <= p.N && (p.ldc & 7) == 0;
+  const bool vec = (p.ldc & 7) == 0;  // then a lane's 8 columns are all inside or all outside
   // bias: past N (and without one) the resource gives zeros
   const __amdgpu_buffer_rsrc_t rbias = make_rsrc(p.bias, p.bias != nullptr ? (long)p.N * 4 : 0);
   float bias[4][4][4];
@@ -492,18 +492,24 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
         }
       const int c = lane & 15, r0 = lane >> 4;
       uint16_t* C = (uint16_t*)p.C + (long)(cm + i * 32 + r0) * p.ldc + cn + c * 8;
-      if (whole) {
+      if (vec) {
+        const int left = cn + c * 8 < p.N ? p.M - cm - i * 32 - r0 : 0;  // rows of this lane still inside
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *(uint4*)(C + (long)q * 4 * p.ldc) = *(const uint4*)(st + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
-      } else {
-        const int nv = min(8, p.N - cn - c * 8);
-#pragma unroll 1
-        for (int q = 0; q < 8 && cm + i * 32 + q * 4 + r0 < p.M; ++q) {
-          const uint16_t* e = (const uint16_t*)(st + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
-#pragma unroll 1
-          for (int k = 0; k < nv; ++k) C[(long)q * 4 * p.ldc + k] = e[k];
+        for (int q = 0; q < 8; ++q) {
+          const uint4 v = *(const uint4*)(st + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
+          if (q * 4 < left) *(uint4*)(C + (long)q * 4 * p.ldc) = v;
         }
+      } else {  // one column a lane, so that a row still leaves in one piece
+        uint16_t* o = (uint16_t*)p.C + (long)(cm + i * 32) * p.ldc + cn + lane;
+        const int left = p.M - cm - i * 32;
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int col = h * 64 + lane;
+            const uint16_t v = *(const uint16_t*)(st + r * 256 + (((col >> 3) ^ (r & 15)) << 4) + (col & 7) * 2);
+            if (r < left && cn + col < p.N) o[(long)r * p.ldc + h * 64] = v;
+          }
       }
       __builtin_amdgcn_sched_barrier(0);
     }

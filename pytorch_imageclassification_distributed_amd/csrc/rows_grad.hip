@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
   // 32 rows x 64 columns at a time, so that a row leaves in 256 contiguous bytes; 16-B chunk c of row r sits at
   // c ^ (r & 15).
   const int cn = n0 + wm * 128, ck = k0 + wn * 128;
-  const bool whole = n0 + 256 <= p.N && k0 + 256 <= p.K && (p.K & 3) == 0;
+  const bool vec = (p.K & 3) == 0;  // then a lane's 4 columns are all inside or all outside
   float* C = p.C + (long)split * p.N * p.K;
   char* so = out[wid];
   const int c = lane & 15, r0 = lane >> 4;
@@ -173,17 +173,20 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
               make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         }
       float* o = C + (long)(cn + i * 32 + r0) * p.K + ck + jj * 64 + c * 4;
-      if (whole) {
+      if (vec) {
+        const int left = ck + jj * 64 + c * 4 < p.K ? p.N - cn - i * 32 - r0 : 0;  // rows of this lane still inside
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *(float4*)(o + (long)q * 4 * p.K) = *(const float4*)(so + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
-      } else {
-        const int nv = min(4, p.K - ck - jj * 64 - c * 4);
-#pragma unroll 1
-        for (int q = 0; q < 8 && cn + i * 32 + q * 4 + r0 < p.N; ++q) {
-          const float* e = (const float*)(so + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
-#pragma unroll 1
-          for (int k = 0; k < nv; ++k) o[(long)q * 4 * p.K + k] = e[k];
+        for (int q = 0; q < 8; ++q) {
+          const float4 v = *(const float4*)(so + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
+          if (q * 4 < left) *(float4*)(o + (long)q * 4 * p.K) = v;
+        }
+      } else {  // one column a lane, so that a row still leaves in one piece
+        float* o1 = C + (long)(cn + i * 32) * p.K + ck + jj * 64 + lane;
+        const int left = p.N - cn - i * 32;
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+          const float v = *(const float*)(so + r * 256 + (((lane >> 2) ^ (r & 15)) << 4) + (lane & 3) * 4);
+          if (r < left && ck + jj * 64 + lane < p.K) o1[(long)r * p.K] = v;
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -196,6 +199,7 @@ __global__ __launch_bounds__(256) void slab_sum_kernel(const float* __restrict__
   const long i = (blockIdx.x * 256L + threadIdx.x) * 4;
   if (i + 4 <= n && (n & 3) == 0) {
     float4 s = *(const float4*)(slabs + i);
+#pragma unroll 8
     for (int k = 1; k < count; ++k) {
       const float4 v = *(const float4*)(slabs + (long)k * n + i);
       s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
@@ -230,7 +234,7 @@ int rows_grad_splits(int M, int N, int K, int ld) {
   const int fewest = (int)((stages + most - 1) / most);
   int best = fewest;
   double least = 1e30;
-  for (int s = fewest; s <= (fewest > 8 ? fewest : 8) && s <= stages; ++s) {
+  for (int s = fewest; s <= (fewest > 64 ? fewest : 64) && s <= stages; ++s) {
     const double t = (double)((tiles * s + 255) / 256) * (1.05 * ((stages + s - 1) / s) + 12) +
                      (s > 1 ? (s + 1) * 4e-6 * N * (double)K / 4 + 3 : 0);
     if (t < least) { least = t; best = s; }
