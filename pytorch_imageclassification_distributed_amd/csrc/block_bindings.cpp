@@ -168,45 +168,26 @@ void rows_sum(Tensor part, Tensor out, int64_t G, int64_t N) {
   ok(rows_sum_launch(part.data_ptr<float>(), out.data_ptr<float>(), (int)G, (int)N, stream_of(part)), "rows_sum");
 }
 
-void quant_rows(Tensor x, OT mask, OT q, OT sc, OT copy, OT part, int64_t M, int64_t N) {
+void quant_rows(Tensor x, Tensor q, Tensor sc, int64_t M, int64_t N) {
   const c10::DeviceGuard guard(x.device());
   const int code = type_code(x, "x");
   dense(x, x, "x");
   TORCH_CHECK(M >= 0 && N >= 1 && N < (1LL << 30) && x.numel() == M * N, "quantize_fp8: shape");
-  like(mask, x, "mask");
-  const int chunk = quant_rows_chunk(M, (int)N);
-  int64_t ldq = 0, ldsc = 0, ldb = 0;
-  if (raw(q)) {
-    TORCH_CHECK(raw(sc), "quantize_fp8: q without scale");
-    blocks(*q, *sc, x, M, N, 1);
-    ldq = q->size(1); ldsc = sc->size(1);
-  }
-  if (raw(copy)) {
-    typed(copy, x, at::kBFloat16, 0, "copy");
-    TORCH_CHECK(copy->dim() == 2 && copy->size(0) == M && copy->size(1) == (N + 7) / 8 * 8, "quantize_fp8: copy shape");
-    ldb = copy->size(1);
-  }
-  typed(part, x, at::kFloat, (M + chunk - 1) / chunk * N, "part");
-  ok(quant_rows_launch(x.data_ptr(), raw(mask), (uint8_t*)raw(q), (uint8_t*)raw(sc), (bf16_t*)raw(copy),
-                       (float*)raw(part), M, (int)N, chunk, ldq, (int)ldsc, (int)ldb, code, stream_of(x)),
+  blocks(q, sc, x, M, N, 1);
+  ok(quant_rows_launch(x.data_ptr(), nullptr, (uint8_t*)q.data_ptr(), sc.data_ptr<uint8_t>(), nullptr, nullptr, M, (int)N,
+                       quant_rows_chunk(M, (int)N), q.size(1), (int)sc.size(1), 0, code, stream_of(x)),
      "quantize_fp8");
 }
 
-void quant_tiles(Tensor w, Tensor q, Tensor sc, OT qt, OT sct) {
+void quant_tiles(Tensor w, Tensor q, Tensor sc) {
   const c10::DeviceGuard guard(w.device());
   const int code = type_code(w, "w");
   dense(w, w, "w");
   TORCH_CHECK(w.dim() == 2 && w.size(0) < (1LL << 23) - 128 && w.size(1) >= 1 && w.size(1) < (1LL << 30),
               "quantize_fp8_weight: shape");
-  const int64_t M = w.size(0), N = w.size(1);
-  blocks(q, sc, w, M, N, 128);
-  if (raw(qt)) {
-    TORCH_CHECK(raw(sct), "quantize_fp8_weight: transpose without scale");
-    blocks(*qt, *sct, w, N, M, 128);
-  }
-  ok(quant_tiles_launch(w.data_ptr(), (uint8_t*)q.data_ptr(), sc.data_ptr<uint8_t>(), (uint8_t*)raw(qt), (uint8_t*)raw(sct),
-                        (int)M, (int)N, q.size(1), (int)sc.size(1), raw(qt) ? qt->size(1) : 0,
-                        raw(qt) ? (int)sct->size(1) : 0, code, stream_of(w)),
+  blocks(q, sc, w, w.size(0), w.size(1), 128);
+  ok(quant_tiles_launch(w.data_ptr(), (uint8_t*)q.data_ptr(), sc.data_ptr<uint8_t>(), nullptr, nullptr, (int)w.size(0),
+                        (int)w.size(1), q.size(1), (int)sc.size(1), 0, 0, code, stream_of(w)),
      "quantize_fp8_weight");
 }
 
@@ -253,7 +234,11 @@ Tensor dense16(const Tensor& t) {
   return ((uintptr_t)c.data_ptr() & 15) == 0 ? c : c.clone();
 }
 OT dense16(const OT& t) { return t.has_value() && t->defined() ? OT(dense16(*t)) : OT(); }
-OT f32(const OT& t) { return t.has_value() && t->defined() ? OT(dense16(t->detach().to(at::kFloat))) : OT(); }
+// a float32 copy where it is not float32 already (only read through its pointer: no gradient flows here)
+OT f32(const OT& t) {
+  if (!t.has_value() || !t->defined()) return OT();
+  return t->scalar_type() == at::kFloat ? dense16(*t) : dense16(t->detach().to(at::kFloat));
+}
 OT some(const Tensor& t) { return t.defined() ? OT(t) : OT(); }
 bool has(const OT& t) { return t.has_value() && t->defined(); }
 Tensor or_undefined(const OT& t) { return has(t) ? *t : Tensor(); }
@@ -274,6 +259,10 @@ struct Slot : torch::CustomClassHolder {
   py::object fn;
   explicit Slot(py::object f) : fn(std::move(f)) {}
   ~Slot() override {
+    if (!Py_IsInitialized()) {  // a graph that outlives the interpreter
+      fn.release();
+      return;
+    }
     py::gil_scoped_acquire gil;
     fn = py::object();
   }
@@ -343,8 +332,8 @@ struct DropoutCounterNode : torch::autograd::Function<DropoutCounterNode> {
 };
 
 Tensor op_dropout_counter(const Tensor& x, const OT& residual, const OT& state, uint64_t seed, uint64_t offset, int64_t t) {
-  if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual)))
-    return drop_forward(x.detach(), residual, state, {t, seed, offset});
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual)))  // nothing asks for a gradient
+    return drop_forward(x, residual, state, {t, seed, offset});
   return DropoutCounterNode::apply(x, residual, state, t, (int64_t)seed, (int64_t)offset);
 }
 
@@ -413,7 +402,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
 std::vector<Tensor> op_rms_norm(const Tensor& x, const OT& residual, const OT& weight, const OT& state, uint64_t seed,
                                 uint64_t offset, int64_t t, double eps, py::object slot) {
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual) || wants(weight))) {
-    RmsOut o = rms_forward(dense16(x.detach()), residual, weight, state, {t, seed, offset}, eps, false);
+    RmsOut o = rms_forward(dense16(x), residual, weight, state, {t, seed, offset}, eps, false);
     if (has(residual)) return {o.y, o.h};
     return {o.y};
   }
@@ -423,7 +412,7 @@ std::vector<Tensor> op_rms_norm(const Tensor& x, const OT& residual, const OT& w
 // (q, scale, h or None)
 std::tuple<Tensor, Tensor, OT> op_rms_norm_fp8(const Tensor& x_, const OT& residual, const OT& weight, double eps) {
   const at::NoGradGuard no_grad;
-  const Tensor x = dense16(x_.detach());
+  const Tensor x = dense16(x_);
   const int64_t n = x.size(-1), rows = x.numel() / n;
   Blocks b = empty_blocks(rows, n, 1, x);
   OT h;
@@ -435,14 +424,14 @@ std::tuple<Tensor, Tensor, OT> op_rms_norm_fp8(const Tensor& x_, const OT& resid
 std::tuple<Tensor, Tensor> op_quantize_rows(const Tensor& x_) {
   const Tensor x = dense16(x_.detach());
   Blocks b = empty_blocks(x.size(0), x.size(1), 1, x);
-  quant_rows(x, OT(), b.q, b.sc, OT(), OT(), x.size(0), x.size(1));
+  quant_rows(x, b.q, b.sc, x.size(0), x.size(1));
   return {b.q, b.sc};
 }
 
 std::tuple<Tensor, Tensor> op_quantize_tiles(const Tensor& w_) {
   const Tensor w = dense16(w_.detach());
   Blocks b = empty_blocks(w.size(0), w.size(1), 128, w);
-  quant_tiles(w, b.q, b.sc, OT(), OT());
+  quant_tiles(w, b.q, b.sc);
   return {b.q, b.sc};
 }
 
@@ -454,51 +443,78 @@ Tensor op_matmul(const Tensor& a, const Tensor& as, const Tensor& b, const Tenso
 }
 
 // dw[n][k] = sum over the m rows of dy[row][n] x[row][k]; dy, x: bf16, widths n, k rounded up to 8
-void rows_grad(const Tensor& dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k) {
+void rows_grad(const bf16_t* dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k) {
   const c10::DeviceGuard guard(dw.device());
   const int64_t ldy = (n + 7) / 8 * 8, ldx = (k + 7) / 8 * 8;
-  typed(dy, dw, at::kBFloat16, m * ldy, "dy");
   typed(x, dw, at::kBFloat16, m * ldx, "x");
   TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.is_contiguous() && dw.numel() == n * k && ((uintptr_t)dw.data_ptr() & 15) == 0,
               "linear_fp8: weight gradient must be contiguous float32");
-  TORCH_CHECK(m < (1LL << 31) - 128, "linear_fp8: too many rows");
   const int splits = rows_grad_splits((int)m, (int)n, (int)k, (int)std::max(ldy, ldx));
   TORCH_CHECK(splits > 0, "linear_fp8: rows too wide for the weight gradient");
   Tensor slabs;
   if (splits > 1) slabs = fresh({splits * n * k}, dw, at::kFloat);
-  ok(rows_grad_launch((const bf16_t*)dy.data_ptr(), (const bf16_t*)x.data_ptr(), dw.data_ptr<float>(),
-                      splits > 1 ? slabs.data_ptr<float>() : nullptr, (int)m, (int)n, (int)k, (int)ldy, (int)ldx, splits,
-                      stream_of(dw)),
+  ok(rows_grad_launch(dy, (const bf16_t*)x.data_ptr(), dw.data_ptr<float>(), splits > 1 ? slabs.data_ptr<float>() : nullptr,
+                      (int)m, (int)n, (int)k, (int)ldy, (int)ldx, splits, stream_of(dw)),
      "linear_fp8 weight gradient");
 }
 
 // y = act(q(x) q(w)^T + b).  Backward: dx = q(dy) q(w) in 8 bits (the weights' transpose was written beside them; 128 x
 // 128 tiles keep their scale), db in float32, and dw = dy^T x on bf16 operands: weight gradients are summed into float32
 // masters over many steps, and the 8-bit matrix instructions cut their sums at 2^-16 where the bf16 ones keep float32.
+// The quantised operands of a call live in one buffer (an allocation costs a small call as much as a launch does).
+struct Layout {
+  int64_t size = 0;
+  int64_t add(int64_t bytes) {
+    const int64_t at = size;
+    size += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+int64_t blocks_of(int64_t cols) { return (cols + 127) / 128; }
+int64_t scales_of(int64_t cols) { return (blocks_of(cols) + 3) / 4 * 4; }
+
 struct LinearOut {
-  Tensor y, xb, wt, wtsc;
+  Tensor y, xb, wt;  // wt: q(w)^T and, behind it, its scales
 };
 LinearOut linear_forward(const Tensor& x, const Tensor& weight, const OT& bias, int64_t act, bool need_x, bool need_w) {
+  const c10::DeviceGuard guard(x.device());
   const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
+  TORCH_CHECK(weight.dim() == 2 && weight.size(1) == k && weight.device() == x.device(), "linear_fp8: weight shape");
+  TORCH_CHECK(m < (1LL << 30) && n >= 1 && n < (1LL << 23) - 128 && k >= 1 && k < (1LL << 23) - 128, "linear_fp8: size");
+  const int tx = type_code(x, "x"), tw = type_code(weight, "weight");
+  const OT b = f32(bias);
+  typed(b, x, at::kFloat, n, "bias");
+  const Tensor w = dense16(weight);
+  dense(x, x, "x"); dense(w, x, "weight");
+  const hipStream_t st = stream_of(x);
+  const int64_t kp = blocks_of(k) * 128, ks = scales_of(k), np = blocks_of(n) * 128, ns = scales_of(n);
   LinearOut o;
-  Blocks a = empty_blocks(m, k, 1, x), b = empty_blocks(n, k, 128, x);
-  OT copy, wt, wtsc;
-  if (need_w) {
-    o.xb = x;
-    if (x.scalar_type() != at::kBFloat16 || k % 8) {
-      o.xb = fresh({m, (k + 7) / 8 * 8}, x, at::kBFloat16);
-      copy = o.xb;
-    }
+  o.xb = x;
+  bf16_t* copy = nullptr;
+  if (need_w && (tx != 0 || k % 8)) {
+    o.xb = fresh({m, (k + 7) / 8 * 8}, x, at::kBFloat16);
+    copy = (bf16_t*)o.xb.data_ptr();
   }
-  quant_rows(x, OT(), a.q, a.sc, copy, OT(), m, k);
+  Layout l;
+  const int64_t aq = l.add(m * kp), as = l.add(m * ks), bq = l.add(n * kp), bs = l.add(blocks_of(n) * ks);
+  const Tensor work = fresh({l.size}, x, at::kByte);
+  uint8_t* p = work.data_ptr<uint8_t>();
+  ok(quant_rows_launch(x.data_ptr(), nullptr, p + aq, p + as, copy, nullptr, m, (int)k, quant_rows_chunk(m, (int)k), kp, (int)ks,
+                       (int)((k + 7) / 8 * 8), tx, st),
+     "linear_fp8");
+  uint8_t *t = nullptr, *ts = nullptr;
   if (need_x) {
-    Blocks t = empty_blocks(k, n, 128, x);
-    o.wt = t.q; o.wtsc = t.sc;
-    wt = t.q; wtsc = t.sc;
+    Layout lt;
+    const int64_t q = lt.add(k * np), sc = lt.add(blocks_of(k) * ns);
+    o.wt = fresh({lt.size}, x, at::kByte);
+    t = o.wt.data_ptr<uint8_t>() + q;
+    ts = o.wt.data_ptr<uint8_t>() + sc;
   }
-  quant_tiles(dense16(weight.detach()), b.q, b.sc, wt, wtsc);
+  ok(quant_tiles_launch(w.data_ptr(), p + bq, p + bs, t, ts, (int)n, (int)k, kp, (int)ks, np, (int)ns, tw, st), "linear_fp8");
   o.y = fresh({m, n}, x, x.scalar_type());
-  fp8_gemm(a.q, a.sc, b.q, b.sc, o.y, f32(bias), k, 128, (int)act);
+  ok(fp8_gemm_launch(p + aq, p + as, p + bq, p + bs, o.y.data_ptr(), (const float*)raw(b), (int)m, (int)n, (int)blocks_of(k), kp,
+                     kp, (int)ks, (int)ks, 7, n, (int)act, tx, st),
+     "linear_fp8");
   return o;
 }
 
@@ -507,7 +523,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
                         bool need_x, bool need_w, c10::IValue wslot, c10::IValue bslot) {
     const Tensor x = dense16(x_);
     LinearOut o = linear_forward(x, weight, bias, act, need_x, need_w);
-    ctx->save_for_backward({o.xb, o.wt, o.wtsc, act ? o.y : Tensor()});
+    ctx->save_for_backward({need_w ? o.xb : Tensor(), o.wt, act ? o.y : Tensor()});
     ctx->saved_data["m"] = x.size(0);
     ctx->saved_data["n"] = weight.size(0);
     ctx->saved_data["k"] = x.size(1);
@@ -520,38 +536,51 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
-    const Tensor &xb = s[0], &wt = s[1], &wtsc = s[2];
-    const OT y = some(s[3]);
+    const Tensor &xb = s[0], &wt = s[1], &y = s[2];
     const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool nb = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
     const Tensor dy = dense16(g[0].detach());
-    Blocks b;
-    Tensor dyb = dy, part, dx, dw, db;
-    OT copy;
-    if (nx) b = empty_blocks(m, n, 1, dy);
-    if (nw && (dy.scalar_type() != at::kBFloat16 || n % 8 || y.has_value())) {
-      dyb = fresh({m, (n + 7) / 8 * 8}, dy, at::kBFloat16);
-      copy = dyb;
-    }
-    if (nb) {
-      const int64_t c = quant_rows_chunk(m, (int)n);
-      part = fresh({(m + c - 1) / c, n}, dy, at::kFloat);
-    }
-    if (nx || copy.has_value() || nb) quant_rows(dy, y, some(b.q), some(b.sc), copy, some(part), m, n);
+    const c10::DeviceGuard guard(dy.device());
+    const int type = type_code(dy, "dy");
+    TORCH_CHECK(dy.dim() == 2 && dy.size(0) == m && dy.size(1) == n, "linear_fp8: dy shape");
+    if (y.defined()) like(OT(y), dy, "y");
+    const hipStream_t st = stream_of(dy);
+    const int64_t np = blocks_of(n) * 128, ns = scales_of(n), n8 = (n + 7) / 8 * 8;
+    const int chunk = quant_rows_chunk(m, (int)n);
+    const int64_t groups = (m + chunk - 1) / chunk;
+    // dy once: 8-bit blocks, a (masked) bf16 copy where dw needs one, partial column sums for db
+    const bool copied = nw && (type != 0 || n % 8 || y.defined());
+    Layout l;
+    const int64_t q = l.add(nx ? m * np : 0), sc = l.add(nx ? m * ns : 0), part = l.add(nb ? groups * n * 4 : 0);
+    const int64_t copy = l.add(copied ? m * n8 * 2 : 0);
+    const Tensor work = fresh({l.size}, dy, at::kByte);
+    uint8_t* p = work.data_ptr<uint8_t>();
+    if (nx || copied || nb)
+      ok(quant_rows_launch(dy.data_ptr(), y.defined() ? y.data_ptr() : nullptr, nx ? p + q : nullptr, nx ? p + sc : nullptr,
+                           copied ? (bf16_t*)(p + copy) : nullptr, nb ? (float*)(p + part) : nullptr, m, (int)n, chunk, np,
+                           (int)ns, (int)n8, type, st),
+         "linear_fp8 backward");
+    Tensor dx, dw, db;
     if (nx) {
       dx = fresh({m, k}, dy, dy.scalar_type());
-      fp8_gemm(b.q, b.sc, wt, wtsc, dx, OT(), n, 128, 0);
+      Layout lt;
+      const int64_t t = lt.add(k * np), ts = lt.add(blocks_of(k) * ns);
+      uint8_t* w = wt.data_ptr<uint8_t>();
+      ok(fp8_gemm_launch(p + q, p + sc, w + t, w + ts, dx.data_ptr(), nullptr, (int)m, (int)k, (int)blocks_of(n), np, np, (int)ns,
+                         (int)ns, 7, k, 0, type, st),
+         "linear_fp8 backward");
     }
     if (nw) {
       dw = slot_or_empty(ctx->saved_data["wslot"], {n, k}, dy);
-      rows_grad(dyb, xb, dw, m, n, k);
+      rows_grad(copied ? (const bf16_t*)(p + copy) : (const bf16_t*)dy.data_ptr(), xb, dw, m, n, k);
       const auto t = (at::ScalarType)ctx->saved_data["wtype"].toInt();
       if (t != at::kFloat) dw = dw.to(t);
     }
     if (nb) {
       db = slot_or_empty(ctx->saved_data["bslot"], {n}, dy);
-      rows_sum(part, db, part.size(0), n);
+      TORCH_CHECK(db.scalar_type() == at::kFloat && db.is_contiguous() && db.numel() == n, "linear_fp8: bias gradient");
+      ok(rows_sum_launch((const float*)(p + part), db.data_ptr<float>(), (int)groups, (int)n, st), "linear_fp8 backward");
       const auto t = (at::ScalarType)ctx->saved_data["btype"].toInt();
       if (t != at::kFloat) db = db.to(t);
     }
@@ -570,7 +599,6 @@ Tensor op_linear_fp8(const Tensor& x, const Tensor& weight, const OT& bias, int6
 }  // namespace
 
 void register_block_ops(pybind11::module& m) {
-  m.def("rms_max_cols", &rms_max_cols);
   m.def("dropout_counter", &op_dropout_counter);
   m.def("rms_norm", &op_rms_norm);
   m.def("rms_norm_fp8", &op_rms_norm_fp8);

@@ -261,59 +261,60 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_fwd_kernel(const T* __restr
   __shared__ float red[16];
   constexpr int RPB = nthreads(TPR) / TPR;
   const int t = threadIdx.x % TPR;
-  const long row = (long)blockIdx.x * RPB + threadIdx.x / TPR;
-  if (RPB > 1 && row >= rows) return;  // whole waves: TPR is 64 where a block holds several rows
   u64 seed = 0, offset = 0;
   if constexpr (DROP) drop_state(d, seed, offset);
-  const long base = row * N;
-  float f[V][8];
-  float s = 0.f;
+  // (a block of several rows holds a wave a row and meets no barrier; otherwise the whole block takes the same rows)
+  for (long row = (long)blockIdx.x * RPB + threadIdx.x / TPR; row < rows; row += (long)gridDim.x * RPB) {
+    const long base = row * N;
+    float f[V][8];
+    float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-    load8<T, VEC>(x + base + c, valid, f[j]);
-    if constexpr (DROP)
-      if (valid > 0) drop8<VEC>(d, seed, offset, base + c, f[j]);
-    if (res != nullptr) {
-      float r[8];
-      load8<T, VEC>(res + base + c, valid, r);
+    for (int j = 0; j < V; ++j) {
+      const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
+      load8<T, VEC>(x + base + c, valid, f[j]);
+      if constexpr (DROP)
+        if (valid > 0) drop8<VEC>(d, seed, offset, base + c, f[j]);
+      if (res != nullptr) {
+        float r[8];
+        load8<T, VEC>(res + base + c, valid, r);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[j][k] += r[k];
-    }
-    if (h != nullptr) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[j][k] = to_f<T>(from_f<T>(f[j][k]));
-      store8<T, VEC>(h + base + c, valid, f[j]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) s += f[j][k] * f[j][k];
-  }
-  s = row_sum<TPR>(s, red);
-  const float inv = 1.f / sqrtf(s / (float)N + eps);
-  if (rstd != nullptr && t == 0) rstd[row] = inv;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-    if (w != nullptr) {
-      float g[8];
-      load8<float, VEC>(w + c, valid, g);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[j][k] *= inv * g[k];
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[j][k] *= inv;
-    }
-    if constexpr (FP8) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k >= valid) f[j][k] = 0.f;  // columns up to the next multiple of 128 are stored as zeros
-      const int e = block_exponent(block_max(f[j]));
-      if (c < ldq) {
-        *(uint2*)(q + row * ldq + c) = to_e4m3x8(f[j], e);
-        if ((t & 15) == 0) put_scale(sc + row * ldsc, c >> 7, (int)(ldq >> 7), ldsc, e);
+        for (int k = 0; k < 8; ++k) f[j][k] += r[k];
       }
-    } else {
-      store8<T, VEC>(y + base + c, valid, f[j]);
+      if (DROP || res != nullptr) {  // what is normalised is h in its own type, stored or not
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[j][k] = to_f<T>(from_f<T>(f[j][k]));
+        if (h != nullptr) store8<T, VEC>(h + base + c, valid, f[j]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += f[j][k] * f[j][k];
+    }
+    s = row_sum<TPR>(s, red);
+    const float inv = 1.f / sqrtf(s / (float)N + eps);
+    if (rstd != nullptr && t == 0) rstd[row] = inv;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
+      if (w != nullptr) {
+        float g[8];
+        load8<float, VEC>(w + c, valid, g);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[j][k] *= inv * g[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[j][k] *= inv;
+      }
+      if constexpr (FP8) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k >= valid) f[j][k] = 0.f;  // columns up to the next multiple of 128 are stored as zeros
+        const int e = block_exponent(block_max(f[j]));
+        if (c < ldq) {
+          *(uint2*)(q + row * ldq + c) = to_e4m3x8(f[j], e);
+          if ((t & 15) == 0) put_scale(sc + row * ldsc, c >> 7, (int)(ldq >> 7), ldsc, e);
+        }
+      } else {
+        store8<T, VEC>(y + base + c, valid, f[j]);
+      }
     }
   }
 }
@@ -639,7 +640,8 @@ int rms_fwd_launch(const void* x, const void* res, const float* w, void* h, void
   BLOCK_TYPE(type, {
     RMS_FWD_SHAPE(N, {
       constexpr int NT = nthreads(TPR);
-      const dim3 grid((unsigned)((rows + NT / TPR - 1) / (NT / TPR)));
+      const long need = (rows + NT / TPR - 1) / (NT / TPR);
+      const dim3 grid((unsigned)(need < (1L << 21) ? need : (1L << 21)));
       auto go = [&](auto vec, auto drop, auto fp8) {
         hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, V, decltype(vec)::value, decltype(drop)::value, decltype(fp8)::value>),
                            grid, dim3(NT), 0, s, (const T*)x, (const T*)res, w, (T*)h, (T*)y, q, sc, rstd, rows, N, ldq,

@@ -27,7 +27,7 @@ def _drop_state(dev, seed, offset):
 
 def _slot(p):
     """What hands out the tensor for ``p``'s float32 gradient, where ``p`` is in a gradient arena."""
-    if p is None or getattr(p, "_imgcls_arena", None) is None or p.dtype != torch.float32 or not p.is_contiguous():
+    if p is None or "_imgcls_arena" not in p.__dict__ or p.dtype != torch.float32 or not p.is_contiguous():
         return None
     return functools.partial(grad_buffer, p, False)
 

@@ -50,9 +50,15 @@ def use_hip(x: torch.Tensor) -> bool:
     return _BACKEND != "torch"
 
 
+_HIP = None
+
+
 def _hip():
-    from . import hip  # noqa: WPS433  (lazy: loads the native extension)
-    return hip
+    global _HIP
+    if _HIP is None:
+        from . import hip  # noqa: WPS433  (lazy: loads the native extension)
+        _HIP = hip
+    return _HIP
 
 
 # ---------------------------------------------------------------------------
@@ -281,19 +287,24 @@ def dropout_counter(x, p, training=True, seed=None, offset=0, residual=None):
     return (y if residual is None else y + residual.float()).to(x.dtype)
 
 
+RMS_MAX_COLS = 32768  # widest row that the HIP kernels keep in registers (csrc/block_ops.hip)
+
+
 def _norm_args(name, x, norm, residual):
     _check_floats(name, x)
     _check_like(name, "residual", residual, x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x needs a last dimension of at least 1, got {tuple(x.shape)}")
-    w = norm.weight
-    if w is not None and (tuple(w.shape) != (x.shape[-1],) or w.device != x.device or w.dtype not in FLOATS):
-        raise ValueError(f"{name}: weight must be [{x.shape[-1]}] on {x.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
-    if w is None and tuple(norm.normalized_shape) != (x.shape[-1],):
-        raise ValueError(f"{name}: the norm is over {tuple(norm.normalized_shape)}, x's rows have {x.shape[-1]}")
-    if use_hip(x) and x.shape[-1] > _hip().C.rms_max_cols():
-        raise ValueError(f"{name}: rows of at most {_hip().C.rms_max_cols()} columns, got {x.shape[-1]}")
-    return w, norm.eps if norm.eps is not None else torch.finfo(x.dtype).eps
+    n = x.shape[-1]
+    w, eps = norm.weight, norm.eps
+    if w is None:
+        if tuple(norm.normalized_shape) != (n,):
+            raise ValueError(f"{name}: the norm is over {tuple(norm.normalized_shape)}, x's rows have {n}")
+    elif w.dim() != 1 or w.shape[0] != n or w.device != x.device or w.dtype not in FLOATS:
+        raise ValueError(f"{name}: weight must be [{n}] on {x.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    if n > RMS_MAX_COLS and use_hip(x):
+        raise ValueError(f"{name}: rows of at most {RMS_MAX_COLS} columns, got {n}")
+    return w, eps if eps is not None else torch.finfo(x.dtype).eps
 
 
 def rms_norm(x, norm, residual=None, p=0.0, training=True, seed=None, offset=0):

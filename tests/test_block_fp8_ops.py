@@ -372,6 +372,18 @@ def test_rms_norm_partial_gradients_and_types(dev):
     assert_within(Fx.rms_norm(x, n0), ref, half(torch.bfloat16) * ref.abs().double() + 1e-5)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("t", TYPES)
+def test_results_do_not_depend_on_asking_for_gradients(dev, t):
+    norm, x, r = norm_case(dev, t, 37, 264, True, 0.3)
+    lin = nn.Linear(264, 40).to(dev)
+    for f in (lambda: Fx.rms_norm(x, norm, p=0.3, seed=4), lambda: Fx.rms_norm(x, norm, residual=r, p=0.3, seed=4)[0],
+              lambda: Fx.dropout_counter(x, 0.3, seed=4, residual=r), lambda: Fx.linear_fp8(x, lin, "relu")):
+        y = f()
+        with torch.no_grad():
+            assert y.requires_grad and torch.equal(f(), y)
+
+
 def test_rms_norm_refuses():
     x, norm = torch.zeros(3, 8), nn.RMSNorm(8)
     with pytest.raises(ValueError):
