@@ -464,7 +464,7 @@ __global__ __launch_bounds__(1024) void rows_sum_kernel(const float* __restrict_
 // ---- quantisation ----
 // rows [M][N] of T -> e4m3 [M][ldq] + E8M0 [M][ldsc], 1 x 128 blocks.  256 threads: 16 rows x 128 columns a step,
 // down `chunk` rows, so the column sums (a bias gradient) come along.  MASK: where ymask <= 0 the value counts as 0
-// (the gradient of a ReLU's input).  COPY: also a bf16 copy with row stride ldb (zeros behind N).
+// (the gradient of a ReLU's input; a NaN there passes it on).  COPY: also a bf16 copy with row stride ldb (zeros behind N).
 template <typename T, bool VEC, bool MASK, bool COPY>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, const T* __restrict__ ymask,
                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ sc,
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
       float y[8];
       load8<T, VEC>(ymask + r * N + c, r < r1 ? valid : 0, y);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = y[k] > 0.f ? f[k] : 0.f;
+      for (int k = 0; k < 8; ++k) f[k] = y[k] <= 0.f ? 0.f : f[k];
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum[k] += f[k];

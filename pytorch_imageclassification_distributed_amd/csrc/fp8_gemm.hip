@@ -48,13 +48,20 @@ DEVI i32x8 frag8(const char* lo, const char* hi) {
   return (i32x8){l.x, l.y, l.z, l.w, h.x, h.y, h.z, h.w};
 }
 
+// a NaN stays one through a ReLU (fmaxf would make it 0)
+template <int ACT>
+DEVI float act_of(float v) {
+  if constexpr (ACT == ACT_RELU) return v < 0.f ? 0.f : v;
+  else return apply_act(v, ACT);
+}
+
 // four consecutive outputs of one row
 template <int ACT, int CT>
 DEVI void store4(const Fp8Gemm& p, int m, int n, const f32x4& v, const float* bias) {
   if (m >= p.M || n >= p.N) return;
   float o[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) o[r] = apply_act(v[r] + bias[r], ACT);
+  for (int r = 0; r < 4; ++r) o[r] = act_of<ACT>(v[r] + bias[r]);
   const long i = (long)m * p.ldc + n;
   if ((p.ldc & 3) == 0 && n + 4 <= p.N) {
     if constexpr (CT == C_F32) *(float4*)((float*)p.C + i) = make_float4(o[0], o[1], o[2], o[3]);
@@ -486,7 +493,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
         for (int g = 0; g < 4; ++g) {
           float v[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = apply_act(acc[i][j][4 * g + r] + bias[j][g][r], ACT);
+          for (int r = 0; r < 4; ++r) v[r] = act_of<ACT>(acc[i][j][4 * g + r] + bias[j][g][r]);
           *(uint2*)(st + fr * 256 + (((j * 4 + g) ^ (fr & 15)) << 4) + fh * 8) = make_uint2(pack_c<CT>(v[0], v[1]), pack_c<CT>(v[2], v[3]));
           if (g == 3) __builtin_amdgcn_sched_barrier(0);
         }

@@ -179,7 +179,7 @@ class _RowsThrough8Bits(torch.autograd.Function):
         x, w, wq, y = ctx.saved_tensors
         g = dy.float()
         if y is not None:
-            g = torch.where(y > 0, g, torch.zeros_like(g))
+            g = torch.where(y <= 0, torch.zeros_like(g), g)
         dx = (dequantize_ref(quantize_rows_ref(g)) @ wq).to(x.dtype)
         dw = (g.bfloat16().float().t() @ x.bfloat16().float()).to(w.dtype)
         return dx, dw, g.sum(0) if ctx.has_b else None, None

@@ -677,6 +677,38 @@ def test_linear_fp8_partial_gradients_shapes_and_parameter_types(dev):
     assert torch.equal(Fx.linear_fp8(x, lin).detach(), before * 2)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("act", [None, "relu", "silu"])
+@pytest.mark.parametrize("m,n", [(3, 40), (70, 200), (600, 520)])
+def test_nan_passes_activations(dev, act, m, n):
+    """A NaN or infinite input makes its row of outputs NaN through every activation, and a ReLU's backward hands such a
+    row's gradient on; the other rows are as without it."""
+    lin = nn.Linear(130, n)
+    with torch.no_grad():
+        lin.weight.copy_(rand((n, 130), torch.float32, "cpu", 87, 0.1))
+    lin = lin.to(dev)
+    x = rand((m, 130), torch.bfloat16, dev, 88)
+    bad = x.clone()
+    bad[1, 7], bad[m - 1, 129] = float("nan"), float("inf")
+    rows = torch.zeros(m, dtype=torch.bool, device=dev)
+    rows[1] = rows[m - 1] = True
+    with torch.no_grad():
+        w = Fx.quantize_fp8_weight(lin.weight)
+        good, got = (Fx.matmul_fp8(Fx.quantize_fp8(v), w, bias=lin.bias, act=act) for v in (x, bad))
+        assert bool(got[rows].isnan().all()) and torch.equal(got[~rows], good[~rows])
+    if act != "silu":
+        dy = rand((m, n), torch.bfloat16, dev, 89)
+        bad.requires_grad_(True)
+        y = Fx.linear_fp8(bad, lin, act)
+        assert bool(y[rows].isnan().all()) and not bool(y[~rows].isnan().any())
+        dx, db = torch.autograd.grad(y, (bad, lin.bias), dy)
+        plain = bad.detach().requires_grad_(True)
+        (through,) = torch.autograd.grad(Fx.linear_fp8(plain, lin), plain, dy)
+        assert torch.equal(dx[rows], through[rows])
+        g = torch.where(y <= 0, 0.0, dy.double()) if act else dy.double()
+        assert_within(db, g.sum(0), (m + 16) * U * g.abs().sum(0), "dbias")
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------
