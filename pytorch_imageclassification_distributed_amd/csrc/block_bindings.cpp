@@ -32,8 +32,9 @@ int quant_rows_launch(const void*, const void*, uint8_t*, uint8_t*, bf16_t*, flo
 int quant_tiles_launch(const void*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, int, int, long, int, long, int, int,
                        hipStream_t);
 int dequant_launch(const uint8_t*, const uint8_t*, void*, long, int, long, int, int, int, hipStream_t);
-int rows_grad_splits(int, int, int, int);
-int rows_grad_launch(const bf16_t*, const bf16_t*, float*, float*, int, int, int, int, int, int, hipStream_t);
+void rows_grad_force(int);
+int rows_grad_plan(int, int, int, int, int*);
+int rows_grad_launch(const bf16_t*, const bf16_t*, float*, float*, int, int, int, int, int, int, int, hipStream_t);
 void fp8_gemm_force(int);
 int fp8_gemm_launch(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, const float*, int, int, int,
                     long, long, int, int, int, long, int, int, hipStream_t);
@@ -449,12 +450,13 @@ void rows_grad(const bf16_t* dy, const Tensor& x, const Tensor& dw, int64_t m, i
   typed(x, dw, at::kBFloat16, m * ldx, "x");
   TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.is_contiguous() && dw.numel() == n * k && ((uintptr_t)dw.data_ptr() & 15) == 0,
               "linear_fp8: weight gradient must be contiguous float32");
-  const int splits = rows_grad_splits((int)m, (int)n, (int)k, (int)std::max(ldy, ldx));
+  int tile = 0;
+  const int splits = rows_grad_plan((int)m, (int)n, (int)k, (int)std::max(ldy, ldx), &tile);
   TORCH_CHECK(splits > 0, "linear_fp8: rows too wide for the weight gradient");
   Tensor slabs;
   if (splits > 1) slabs = fresh({splits * n * k}, dw, at::kFloat);
   ok(rows_grad_launch(dy, (const bf16_t*)x.data_ptr(), dw.data_ptr<float>(), splits > 1 ? slabs.data_ptr<float>() : nullptr,
-                      (int)m, (int)n, (int)k, (int)ldy, (int)ldx, splits, stream_of(dw)),
+                      (int)m, (int)n, (int)k, (int)ldy, (int)ldx, tile, splits, stream_of(dw)),
      "linear_fp8 weight gradient");
 }
 
@@ -611,4 +613,5 @@ void register_block_ops(pybind11::module& m) {
   });
   m.def("linear_fp8", &op_linear_fp8);
   m.def("fp8_gemm_force", &fp8_gemm_force);
+  m.def("rows_grad_force", &rows_grad_force);
 }

@@ -429,6 +429,14 @@ DEVI void wait_vmcnt() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | (((N >> 4) & 3) << 14));
 }
 
+// vmcnt(N) and lgkmcnt(0): before a barrier behind which other waves overwrite what this wave has read from LDS (the
+// matrix instructions that use it, and hipcc's waits with them, may be scheduled past the barrier)
+template <int N>
+DEVI void wait_vmcnt_lds() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (((N >> 4) & 3) << 14));
+}
+
 DEVI void glds16(const void* src, char* lds_wave_base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }

@@ -159,10 +159,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
   // stage takes tile kt + S - 1
   auto step = [&](auto c, int kt) __attribute__((always_inline)) {
     constexpr int U = decltype(c)::value;
-    wait_vmcnt<(S - 2) * LPS>();
+    wait_vmcnt_lds<(S - 2) * LPS>();
     __builtin_amdgcn_s_barrier();
     issue(kt + S - 1, stage(std::integral_constant<int, U + S - 1>{}));
-    if ((kt & 3) == 0) {
+    if (S == 4 ? U == 0 : (kt & 3) == 0) {
       const int nxt = min((kt >> 2) + 1, (nk - 1) >> 2);
 #pragma unroll
       for (int i = 0; i < RM; ++i) { sx[i] = nx[i]; nx[i] = ssa[i][nxt]; }
@@ -198,16 +198,24 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
     issue(1, s1);
     issue(2, s2);
   }
-  for (int kt = 0;;) {
+  // (whole rounds of the ring, then the rest: with exits inside the loop hipcc joins their states at its head, and waits
+  // for every load there)
+  int kt = 0;
+  for (; kt + S <= nk; kt += S) {
     step(std::integral_constant<int, 0>{}, kt);
-    if (++kt >= nk) break;
-    step(std::integral_constant<int, 1>{}, kt);
-    if (++kt >= nk) break;
+    step(std::integral_constant<int, 1>{}, kt + 1);
     if constexpr (S == 4) {
-      step(std::integral_constant<int, 2>{}, kt);
-      if (++kt >= nk) break;
-      step(std::integral_constant<int, 3>{}, kt);
-      if (++kt >= nk) break;
+      step(std::integral_constant<int, 2>{}, kt + 2);
+      step(std::integral_constant<int, 3>{}, kt + 3);
+    }
+  }
+  if (kt < nk) {
+    step(std::integral_constant<int, 0>{}, kt);
+    if constexpr (S == 4) {
+      if (kt + 1 < nk) {
+        step(std::integral_constant<int, 1>{}, kt + 1);
+        if (kt + 2 < nk) step(std::integral_constant<int, 2>{}, kt + 2);
+      }
     }
   }
   wait_vmcnt<0>();
@@ -538,13 +546,13 @@ int g_force = -1;  // tests and measurements: run this kernel whatever the sizes
 // Which kernel: the one whose time this estimates lowest, in us, from what each measured on 256 CUs - a round of blocks
 // costs so much a k-step, plus its first loads and its outputs.  Measured (K 4096 unless given; kernel: us):
 //   16 x 4096        few16 7.0   64x64 10.2   128x64 -     128x128(4) -     128x128(2) 29   256 46
-//   32 x 4096        few32 9.6   64x64 10.6
-//   64 x 4096        few32 16.6  64x64 11.2
-//   512 x 4096                   64x64 23.0   128x64 18.2  128x128(4) 24.1  128x128(2) 34   256 41
-//   1024 x 4096                  64x64 42.8   128x64 33.9  128x128(4) 28.4  128x128(2) 36   256 41
-//   2048 x 4096                  64x64 82.7   128x64 73.5  128x128(4) 59.0  128x128(2) 50   256 57
-//   4096 x 4096                  64x64 161    128x64 146   128x128(4) 117   128x128(2) 98   256 65
-//   8192 x 2048, K 512           64x64 37.5   128x64 41.9  128x128(4) 34.5  128x128(2) 26   256 19
+//   32 x 4096        few32 9.7   64x64 10.2
+//   64 x 4096        few32 16.4  64x64 11.1
+//   512 x 4096                   64x64 22.8   128x64 19.0  128x128(4) 24.1  128x128(2) 32   256 42
+//   1024 x 4096                  64x64 42.2   128x64 35.1  128x128(4) 27.0  128x128(2) 35   256 42
+//   2048 x 4096                  64x64 82.6   128x64 73.6  128x128(4) 57.2  128x128(2) 50   256 58
+//   4096 x 4096                  64x64 161    128x64 147   128x128(4) 113   128x128(2) 101  256 65
+//   8192 x 2048, K 512           64x64 37.0   128x64 41.2  128x128(4) 33.1  128x128(2) 25   256 19
 enum { K_FEW16, K_FEW32, K_64, K_128x64, K_128_4, K_128_2, K_256, K_COUNT };
 
 double estimate(int k, const Fp8Gemm& p) {

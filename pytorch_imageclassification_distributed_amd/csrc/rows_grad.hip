@@ -10,7 +10,7 @@
 //   second half (B 2, 3): the stage after next goes into this buffer; B 0, 1 and, block by block, A of the next stage are
 //                         read from the other one.
 // Bound by the matrix pipe at the clock that it can hold: 8192 x 8192 x 4096 in 420 us (1.3 PFLOP/s), 65536 rows of
-// 512 x 512 in 50 us, 1024 x 1000 x 2048 in 25 us (few output tiles: the rows are split, and the slabs added in order).
+// 512 x 512 in 50 us (few output tiles: the rows are split, and the slabs added in order).
 #include <type_traits>
 
 #include "conv_common.h"
@@ -34,6 +34,42 @@ DEVI void mma(f32x16_t& acc, const bf16x8& b, const bf16x8& a) {
 
 DEVI void dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, int soff, char* lds_wave_base) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds_wave_base, 16, voff, soff, 0, 0);
+}
+
+// a fragment's 8 rows of a column: two transposing reads of four rows each, `next` bytes apart
+DEVI bf16x8 tr_frag(char* at, int next) {
+  const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_t*)at);
+  const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_t*)(at + next));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// 32 x 64 outputs at (row, col): v0 the left 32 columns, v1 the right; v[4 g + r] is row fr, column 8 g + 4 fh + r.  They
+// pass through 8 KB of the wave's own LDS, so that a row leaves in 256 contiguous bytes; 16-B chunk c of row r sits at
+// c ^ (r & 15).
+DEVI void put_32x64(char* so, const f32x16_t& v0, const f32x16_t& v1, float* C, int N, int K, int row, int col, int lane) {
+  const int fr = lane & 31, fh = lane >> 5, c = lane & 15, r0 = lane >> 4;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    *(float4*)(so + fr * 256 + (((g * 2 + fh) ^ (fr & 15)) << 4)) = make_float4(v0[4 * g], v0[4 * g + 1], v0[4 * g + 2], v0[4 * g + 3]);
+    *(float4*)(so + fr * 256 + (((8 + g * 2 + fh) ^ (fr & 15)) << 4)) = make_float4(v1[4 * g], v1[4 * g + 1], v1[4 * g + 2], v1[4 * g + 3]);
+  }
+  if ((K & 3) == 0) {  // then a lane's 4 columns are all inside or all outside
+    float* o = C + (long)(row + r0) * K + col + c * 4;
+    const int left = col + c * 4 < K ? N - row - r0 : 0;  // rows of this lane still inside
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 v = *(const float4*)(so + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
+      if (q * 4 < left) *(float4*)(o + (long)q * 4 * K) = v;
+    }
+  } else {  // one column a lane, so that a row still leaves in one piece
+    float* o = C + (long)row * K + col + lane;
+    const int left = N - row;
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r) {
+      const float v = *(const float*)(so + r * 256 + (((lane >> 2) ^ (r & 15)) << 4) + (lane & 3) * 4);
+      if (r < left && col + lane < K) o[(long)r * K] = v;
+    }
+  }
 }
 
 constexpr int STAGE_ROWS = 64, ROW_BYTES = 512, IMAGE = STAGE_ROWS * ROW_BYTES;
@@ -81,7 +117,7 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
   // fragment (block i of 32 columns, quarter s of 16 rows): lane l holds column l & 31, rows 8 (l >> 5) + 0 .. 7 of the
   // quarter, four rows a transposing read: 16 lanes read 4 rows x 16 columns, lane (tq, tp) 8 bytes of row tq, and
   // receive a column each
-  const int fr = lane & 31, fh = lane >> 5;
+  const int fh = lane >> 5;
   const int tq = (lane & 15) >> 2, tp = lane & 3, half16 = (lane >> 4) & 1;
   const int row0 = 8 * fh + tq;  // + 16 s + 4 e: the swizzle depends on tq alone
   int oa[4], ob[4];
@@ -91,9 +127,7 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
     ob[i] = IMAGE + row0 * ROW_BYTES + (((wn * 8 + i * 2 + half16) ^ (tq << 1)) << 5) + tp * 8;
   }
   auto frag = [&](char* buf, int o, int s) __attribute__((always_inline)) {
-    const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_t*)(buf + o + s * 16 * ROW_BYTES));
-    const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) bf16x4_t*)(buf + o + (s * 16 + 4) * ROW_BYTES));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return tr_frag(buf + o + s * 16 * ROW_BYTES, 4 * ROW_BYTES);
   };
 
   f32x16_t acc[4][4];
@@ -153,45 +187,123 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
     asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]));
   wait_vmcnt<0>();  // (LDS-DMA must not outlive the block)
 
-  // acc[i][j][4 g + r]: row 32 i + fr, column 32 j + 8 g + 4 fh + r of the wave's 128 x 128.  Through the wave's own LDS,
-  // 32 rows x 64 columns at a time, so that a row leaves in 256 contiguous bytes; 16-B chunk c of row r sits at
-  // c ^ (r & 15).
   const int cn = n0 + wm * 128, ck = k0 + wn * 128;
-  const bool vec = (p.K & 3) == 0;  // then a lane's 4 columns are all inside or all outside
   float* C = p.C + (long)split * p.N * p.K;
-  char* so = out[wid];
-  const int c = lane & 15, r0 = lane >> 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const f32x16_t& v = acc[i][jj * 2 + j];
-          *(float4*)(so + fr * 256 + (((j * 8 + g * 2 + fh) ^ (fr & 15)) << 4)) =
-              make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
-        }
-      float* o = C + (long)(cn + i * 32 + r0) * p.K + ck + jj * 64 + c * 4;
-      if (vec) {
-        const int left = ck + jj * 64 + c * 4 < p.K ? p.N - cn - i * 32 - r0 : 0;  // rows of this lane still inside
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 v = *(const float4*)(so + (q * 4 + r0) * 256 + ((c ^ ((q * 4 + r0) & 15)) << 4));
-          if (q * 4 < left) *(float4*)(o + (long)q * 4 * p.K) = v;
-        }
-      } else {  // one column a lane, so that a row still leaves in one piece
-        float* o1 = C + (long)(cn + i * 32) * p.K + ck + jj * 64 + lane;
-        const int left = p.N - cn - i * 32;
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-          const float v = *(const float*)(so + r * 256 + (((lane >> 2) ^ (r & 15)) << 4) + (lane & 3) * 4);
-          if (r < left && ck + jj * 64 + lane < p.K) o1[(long)r * p.K] = v;
-        }
-      }
+      put_32x64(out[wid], acc[i][jj * 2], acc[i][jj * 2 + 1], C, p.N, p.K, cn + i * 32, ck + jj * 64, lane);
       __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// ---- the small tile ----
+// 128 x 128 outputs on 4 waves of 64 x 64, for gradients of few outputs over few rows: four times the blocks of the large
+// tile.  A ring of four 32 KB stages of 64 rows, three in flight, since a wave's 16 MFMAs a stage (512 cycles) are
+// shorter than the way to memory.  Bound by the LDS port (a stage is 32 KB in and 64 KB out, 96 KB at 128 B a cycle = 770
+// cycles) and, for few stages, by the first loads and the outputs.  small / large tile: 1024 x 1000 x 2048 13.2 / 24.6 us,
+// 2048 x 2048 x 2048 23.8 / 36.6, 65536 x 512 x 512 42 / 50, 4096 x 4096 x 4096 162 / 105.
+__global__ __launch_bounds__(256, 1) void rows_grad_small_kernel(const RowsGrad p) {
+  constexpr int PITCH = 256, IMG = STAGE_ROWS * PITCH, PIECES = 8;
+  __shared__ __attribute__((aligned(16))) char s0[2 * IMG];  // (separate arrays: as above)
+  __shared__ __attribute__((aligned(16))) char s1[2 * IMG];
+  __shared__ __attribute__((aligned(16))) char s2[2 * IMG];
+  __shared__ __attribute__((aligned(16))) char s3[2 * IMG];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid >> 1, wn = wid & 1;
+  const int gm = (p.N + 127) >> 7, gn = (p.K + 127) >> 7, tiles = gm * gn;
+  const int all = xcd_remap(blockIdx.x, gridDim.x), split = all / tiles, lin = all - split * tiles;
+  const int n0 = __builtin_amdgcn_readfirstlane(lin / gn * 128), k0 = __builtin_amdgcn_readfirstlane(lin % gn * 128);
+  const int m0 = __builtin_amdgcn_readfirstlane(split * p.rows), nrows = min(p.M - m0, p.rows);
+  const int stages = (nrows + STAGE_ROWS - 1) / STAGE_ROWS;
+
+  // rows past this split's end are past the resource: zeros, also for the stages behind the last
+  const __amdgpu_buffer_rsrc_t ry = make_rsrc(p.Y + (long)m0 * p.ldy + n0, 2 * ((long)nrows * p.ldy - n0));
+  const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.X + (long)m0 * p.ldx + k0, 2 * ((long)nrows * p.ldx - k0));
+  // piece q of a wave: rows 16 wid + 4 q .. + 3 of an image, lane l chunk l & 15 of row l >> 4; swizzle as above
+  const int pr = lane >> 4, ch = lane & 15;
+  const int src = (((ch >> 1) ^ (pr << 1)) << 5) + ((ch & 1) << 4);
+  const int sy = 2 * p.ldy, sx = 2 * p.ldx;
+  const unsigned vy = (unsigned)((wid * 16 + pr) * sy + src), vx = (unsigned)((wid * 16 + pr) * sx + src);
+  auto issue = [&](int st, char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) dma16(ry, vy, (st * STAGE_ROWS + q * 4) * sy, buf + (wid * 16 + q * 4) * PITCH);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) dma16(rx, vx, (st * STAGE_ROWS + q * 4) * sx, buf + IMG + (wid * 16 + q * 4) * PITCH);
+  };
+  auto ring = [&](auto c) __attribute__((always_inline)) -> char* {
+    constexpr int U = decltype(c)::value % 4;
+    if constexpr (U == 0) return s0;
+    else if constexpr (U == 1) return s1;
+    else if constexpr (U == 2) return s2;
+    else return s3;
+  };
+
+  const int fh = lane >> 5, tq = (lane & 15) >> 2, tp = lane & 3, half16 = (lane >> 4) & 1;
+  int oa[2], ob[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    oa[i] = (8 * fh + tq) * PITCH + (((wm * 4 + i * 2 + half16) ^ (tq << 1)) << 5) + tp * 8;
+    ob[i] = IMG + (8 * fh + tq) * PITCH + (((wn * 4 + i * 2 + half16) ^ (tq << 1)) << 5) + tp * 8;
+  }
+  f32x16_t acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x16_t{};
+
+  // stage st = 4 n + U: it has landed (two younger ones are in flight), every wave has left stage st - 1, whose buffer
+  // takes stage st + 3
+  auto step = [&](auto c, int st) __attribute__((always_inline)) {
+    constexpr int U = decltype(c)::value;
+    wait_vmcnt_lds<2 * PIECES>();
+    __builtin_amdgcn_s_barrier();
+    issue(st + 3, ring(std::integral_constant<int, U + 3>{}));
+    char* buf = ring(c);
+    bf16x8 a[2][4], b[2][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        a[i][s] = tr_frag(buf + oa[i] + s * 16 * PITCH, 4 * PITCH);
+        b[i][s] = tr_frag(buf + ob[i] + s * 16 * PITCH, 4 * PITCH);
+      }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j][s], a[i][s], acc[i][j], 0, 0, 0);
+  };
+  issue(0, s0);
+  issue(1, s1);
+  issue(2, s2);
+  // (whole rounds of the ring, then the rest: with exits inside the loop hipcc joins their states at its head, and waits
+  // for every load there)
+  int st = 0;
+  for (; st + 4 <= stages; st += 4) {
+    step(std::integral_constant<int, 0>{}, st);
+    step(std::integral_constant<int, 1>{}, st + 1);
+    step(std::integral_constant<int, 2>{}, st + 2);
+    step(std::integral_constant<int, 3>{}, st + 3);
+  }
+  if (st < stages) {
+    step(std::integral_constant<int, 0>{}, st);
+    if (st + 1 < stages) {
+      step(std::integral_constant<int, 1>{}, st + 1);
+      if (st + 2 < stages) step(std::integral_constant<int, 2>{}, st + 2);
+    }
+  }
+  wait_vmcnt<0>();
+  __syncthreads();  // s0 holds outputs now
+  float* C = p.C + (long)split * p.N * p.K;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    put_32x64(s0 + wid * 8192, acc[i][0], acc[i][1], C, p.N, p.K, n0 + wm * 64 + i * 32, k0 + wn * 64, lane);
+    __builtin_amdgcn_sched_barrier(0);
+  }
 }
 
 // out = the sum of the slabs, in order
@@ -223,22 +335,32 @@ int stages_of(int M) { return (M + STAGE_ROWS - 1) / STAGE_ROWS; }
 
 }  // namespace
 
-// Row splits: few tiles over many rows leave CUs idle, slabs cost their bytes twice.  Estimated time in us: a round of
-// 256 blocks takes 1.05 a stage and 12 for first loads and outputs; the slabs' sum 4 TB/s.  At least as many as keep the
-// byte offsets inside a split (and the three stages past its end) in 32 bits.
-int rows_grad_splits(int M, int N, int K, int ld) {
-  const long tiles = (long)cdiv(N, 256) * cdiv(K, 256);
+static int g_force = 0;  // tests: this tile whatever the sizes (rows_grad_force)
+void rows_grad_force(int tile) { g_force = tile; }
+
+// The tile's width and the row splits: few tiles over few rows leave CUs idle, slabs cost their bytes twice.  Estimated
+// time in us: a round of 256 blocks takes 1.45 a stage and 14 for first loads and outputs, with the small tile 0.5 and 7
+// (4096 x 4096 x 4096: 105 and 162 us; 300 x 4096 x 4096: 22 and 31; 4096 x 2048 x 2048: 50 and 38); the slabs' sum
+// 4 TB/s.  At least as many splits as keep the byte offsets inside one (and the three stages past its end) in 32 bits; 0
+// where even the shortest split is too long.
+int rows_grad_plan(int M, int N, int K, int ld, int* tile) {
   const int stages = stages_of(M);
+  *tile = 256;
   if (stages == 0) return 1;
   const long most = ((1L << 31) - 1) / (2L * STAGE_ROWS * ld) - 4;  // stages a split can hold
   if (most < 1) return 0;
   const int fewest = (int)((stages + most - 1) / most);
   int best = fewest;
   double least = 1e30;
-  for (int s = fewest; s <= (fewest > 64 ? fewest : 64) && s <= stages; ++s) {
-    const double t = (double)((tiles * s + 255) / 256) * (1.05 * ((stages + s - 1) / s) + 12) +
-                     (s > 1 ? (s + 1) * 4e-6 * N * (double)K / 4 + 3 : 0);
-    if (t < least) { least = t; best = s; }
+  for (int t = 128; t <= 256; t += 128) {
+    if (g_force && g_force != t) continue;
+    const long tiles = (long)cdiv(N, t) * cdiv(K, t);
+    for (int s = fewest; s <= (fewest > 64 ? fewest : 64) && s <= stages; ++s) {
+      const double rounds = (double)((tiles * s + 255) / 256), per = (stages + s - 1) / s;
+      const double us = rounds * (t == 256 ? 1.45 * per + 14 : 0.5 * per + 7) +
+                        (s > 1 ? (s + 1) * 4e-6 * N * (double)K / 4 + 3 : 0);
+      if (us < least) { least = us; best = s; *tile = t; }
+    }
   }
   const int per = (stages + best - 1) / best;  // no empty split
   return (stages + per - 1) / per;
@@ -246,7 +368,7 @@ int rows_grad_splits(int M, int N, int K, int ld) {
 
 // slabs: float32 [splits][N][K], used where splits > 1
 int rows_grad_launch(const bf16_t* Y, const bf16_t* X, float* C, float* slabs, int M, int N, int K, int ldy, int ldx,
-                     int splits, hipStream_t s) {
+                     int tile, int splits, hipStream_t s) {
   if (N <= 0 || K <= 0) return 0;
   const long n = (long)N * K;
   if (M <= 0) {
@@ -255,12 +377,13 @@ int rows_grad_launch(const bf16_t* Y, const bf16_t* X, float* C, float* slabs, i
     return 0;
   }
   const int stages = stages_of(M), per = (stages + splits - 1) / splits;
-  const long tiles = (long)cdiv(N, 256) * cdiv(K, 256);
-  if ((per + 4L) * STAGE_ROWS * 2 * (ldy > ldx ? ldy : ldx) >= (1L << 31) || (splits - 1L) * per >= stages ||
+  const long tiles = (long)cdiv(N, tile) * cdiv(K, tile);
+  if ((tile != 128 && tile != 256) || (per + 4L) * STAGE_ROWS * 2 * (ldy > ldx ? ldy : ldx) >= (1L << 31) || (splits - 1L) * per >= stages ||
       tiles * splits >= (1L << 31) || (splits > 1 && slabs == nullptr))
     return (int)hipErrorInvalidValue;
   const RowsGrad p{Y, X, splits > 1 ? slabs : C, M, N, K, ldy, ldx, per * STAGE_ROWS};
-  hipLaunchKernelGGL(rows_grad_kernel, dim3((unsigned)(tiles * splits)), dim3(256), 0, s, p);
+  if (tile == 256) hipLaunchKernelGGL(rows_grad_kernel, dim3((unsigned)(tiles * splits)), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL(rows_grad_small_kernel, dim3((unsigned)(tiles * splits)), dim3(256), 0, s, p);
   HIP_CHECK_LAUNCH();
   if (splits > 1) {
     hipLaunchKernelGGL(slab_sum_kernel, dim3((unsigned)((n / 4 + 256) / 256)), dim3(256), 0, s, slabs, C, n, splits);

@@ -646,6 +646,24 @@ def test_linear_fp8(dev, t, m, k, n, act, bias):
         assert_within(grads[2], g.sum(0), (m + 16) * U * g.abs().sum(0) + 1e-30, "dbias")
 
 
+@gpu
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("m,n,k", [(1, 5, 7), (63, 130, 129), (64, 128, 128), (65, 257, 300), (192, 100, 1281), (257, 384, 515), (320, 64, 256),
+                                   (1024, 127, 640), (9000, 40, 72)])
+def test_linear_fp8_weight_gradient_tiles(tile, m, n, k):
+    """Both weight-gradient kernels at sizes around their tiles, stages and row splits.  Integers: every sum is exact."""
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    g = torch.Generator().manual_seed(m + n + k)
+    lin = nn.Linear(k, n).to("cuda")
+    x, dy = (torch.randint(-4, 5, (m, c), generator=g).to(torch.bfloat16) for c in (k, n))
+    try:
+        hip.C.rows_grad_force(tile)
+        (dw,) = torch.autograd.grad(Fx.linear_fp8(x.cuda(), lin), (lin.weight,), dy.cuda())
+    finally:
+        hip.C.rows_grad_force(0)
+    assert torch.equal(dw.double().cpu(), dy.double().t() @ x.double())
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 def test_linear_fp8_partial_gradients_shapes_and_parameter_types(dev):
     lin = nn.Linear(72, 24).to(dev)
