@@ -400,9 +400,9 @@ def linear_fp8(x, lin, act=None):
         raise ValueError(f"linear_fp8: weight {w.dtype} {tuple(w.shape)}")
     if w.device != x.device or (b is not None and b.device != x.device):
         raise ValueError(f"linear_fp8: x on {x.device}, weight on {w.device}")
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])  # (a reshape or view is an autograd node more, 8 us a call)
     y = _hip().linear_fp8(x2, w, b, act) if use_hip(x) else linear_fp8_ref(x2, w, b, act)
-    return y.view(*x.shape[:-1], w.shape[0])
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.shape[0])
 
 
 class ConcatPlan:
