@@ -3,14 +3,14 @@
 Layout:
 * ``csrc/*.hip``      - kernels + ``extern "C"``-free C++ launchers; include only
                         HIP headers, so each TU compiles in seconds;
-* ``csrc/bindings.cpp`` - the only TU that includes torch headers: argument
-                        checking, allocation through the caching allocator,
-                        current-stream lookup, pybind11 module ``_C``.
+* ``csrc/bindings.cpp``, ``csrc/block_bindings.cpp`` - the TUs that include torch
+                        headers: argument checking, allocation through the
+                        caching allocator, current-stream lookup, autograd nodes
+                        of the 8-bit linear block, pybind11 module ``_C``.
 
 Objects are cached in ``build/`` by content hash of the source + flags, so an
 unchanged kernel file is not recompiled.  The result
-``pytorch_imageclassification_distributed_amd/_C.so`` is git-ignored but travels
-to the GPU box with the gpurun snapshot.
+``pytorch_imageclassification_distributed_amd/_C.so`` is git-ignored.
 """
 from __future__ import annotations
 

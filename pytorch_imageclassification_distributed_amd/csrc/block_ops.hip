@@ -26,35 +26,89 @@ struct alignas(16) Pack8 {
   T e[8];
 };
 
-// the same 8 elements at any address that a T may have: one access as well (the hardware splits it where it must)
+// 8 elements as loaded (half the registers of their float values in a 16-bit type)
+template <typename T>
+struct Raw8 {
+  static constexpr int W = (int)sizeof(T) * 2;
+  uint32_t w[W];
+  DEVI float get(int k) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
+    else if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k >> 1] >> (16 * (k & 1))));
+  }
+  // forget that the float values are known: they are made again where they are used next, not kept in registers
+  DEVI void launder() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
+  }
+};
+
+// The same at any address that a T may have: one access as well (the hardware splits it where it must).
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Loose8 {
   T e[8];
 };
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// 8 consecutive elements, `valid` of them inside the row.  VEC: whole aligned vectors (valid is 0 or 8).  Otherwise a row
-// may begin at any element and only its last vector is cut: by elements alone, 16384 x 4095 took four times as long as
-// 16384 x 4096.
+// 8 consecutive elements of a row from column c on, `valid` of them inside it, as they come from memory.  VEC: rows of
+// whole aligned vectors (valid is 0 or 8).  Otherwise a row may begin at any element (by elements alone, 16384 x 4095 took
+// four times as long as 16384 x 4096), and its last vector is cut.  In a 16-bit type that vector is the 8 elements that end
+// with the row, and settle8 shifts it down, zeros behind (a row shorter than 8 is read by elements): guarded loads of one
+// element follow each other, and a wait stands between each (16384 x 4095 bf16 norm, forward + backward: 144 + 220 us
+// against 124 + 137).  In float32 the shift costs more than they do (264 + 197 us against 239 + 168).
 template <typename T, bool VEC>
-DEVI void load8(const T* p, int valid, float* f) {
+DEVI Raw8<T> raw8(const T* p, long c, int valid) {
+  Raw8<T> v;
+#pragma unroll
+  for (int i = 0; i < Raw8<T>::W; ++i) v.w[i] = 0u;
   if constexpr (VEC) {
     if (valid > 0) {
-      const Pack8<T> v = *(const Pack8<T>*)p;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = to_f<T>(v.e[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = 0.f;
+      for (int i = 0; i < Raw8<T>::W; i += 4) {
+        const uint4 u = ((const uint4*)p)[i >> 2];
+        v.w[i] = u.x; v.w[i + 1] = u.y; v.w[i + 2] = u.z; v.w[i + 3] = u.w;
+      }
     }
+  } else if (valid == 8 || (sizeof(T) == 2 && valid > 0 && c > 0)) {
+    const Loose8<T> l = *(const Loose8<T>*)(p + (valid - 8));
+    __builtin_memcpy(v.w, l.e, sizeof(l));
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 7; ++k) v.w[k] = k < valid ? __float_as_uint(p[k]) : 0u;
+  } else if (valid > 0) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k)  // place k holds element k + valid - 8, as in the vector that ends with a longer row
+      if (k + valid >= 8) v.w[k >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[k + valid - 8]) << (16 * (k & 1));
+  }
+  return v;
+}
+
+template <typename T, bool VEC>
+DEVI void settle8(Raw8<T>& r, int valid) {
+  if constexpr (!VEC && sizeof(T) == 2) {
+    const int d = (8 - valid) & 7;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    u32x4 a = {r.w[0], r.w[1], r.w[2], r.w[3]};
+    a = d & 4 ? __builtin_shufflevector(a, zero, 2, 3, 4, 5) : a;
+    a = d & 2 ? __builtin_shufflevector(a, zero, 1, 2, 3, 4) : a;
+    const unsigned sh = (unsigned)(d & 1) * 16;
+    r.w[0] = __builtin_amdgcn_alignbit(a[1], a[0], sh);
+    r.w[1] = __builtin_amdgcn_alignbit(a[2], a[1], sh);
+    r.w[2] = __builtin_amdgcn_alignbit(a[3], a[2], sh);
+    r.w[3] = __builtin_amdgcn_alignbit(0u, a[3], sh);
+  }
+}
+
+template <typename T, bool VEC>
+DEVI void load8(const T* p, long c, int valid, float* f) {
+  if (valid > 0 || (!VEC && sizeof(T) == 4)) {  // (guarded loads need no branch around them)
+    Raw8<T> v = raw8<T, VEC>(p, c, valid);
+    settle8<T, VEC>(v, valid);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = v.get(k);
   } else {
-    if (valid == 8) {
-      const Loose8<T> v = *(const Loose8<T>*)p;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = to_f<T>(v.e[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = k < valid ? to_f<T>(p[k]) : 0.f;
-    }
+    for (int k = 0; k < 8; ++k) f[k] = 0.f;
   }
 }
 
@@ -79,50 +133,6 @@ DEVI void store8(T* p, int valid, const float* f) {
         if (k < valid) p[k] = from_f<T>(f[k]);
     }
   }
-}
-
-// 8 elements as loaded (half the registers of their float values in a 16-bit type)
-template <typename T>
-struct Raw8 {
-  static constexpr int W = (int)sizeof(T) * 2;
-  uint32_t w[W];
-  DEVI float get(int k) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[k]);
-    else if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(k & 1 ? w[k >> 1] & 0xffff0000u : w[k >> 1] << 16);
-    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[k >> 1] >> (16 * (k & 1))));
-  }
-  // forget that the float values are known: they are made again where they are used next, not kept in registers
-  DEVI void launder() {
-#pragma unroll
-    for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
-  }
-};
-
-template <typename T, bool VEC>
-DEVI Raw8<T> raw8(const T* p, int valid) {
-  Raw8<T> v;
-  if constexpr (VEC) {
-#pragma unroll
-    for (int i = 0; i < Raw8<T>::W; i += 4) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (valid > 0) u = ((const uint4*)p)[i >> 2];
-      v.w[i] = u.x; v.w[i + 1] = u.y; v.w[i + 2] = u.z; v.w[i + 3] = u.w;
-    }
-  } else if (valid == 8) {
-    const Loose8<T> u = *(const Loose8<T>*)p;
-    __builtin_memcpy(v.w, u.e, sizeof(u));
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v.w[k] = k < valid ? __float_as_uint(p[k]) : 0u;
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t lo = 2 * k < valid ? __builtin_bit_cast(uint16_t, p[2 * k]) : 0u;
-      const uint32_t hi = 2 * k + 1 < valid ? __builtin_bit_cast(uint16_t, p[2 * k + 1]) : 0u;
-      v.w[k] = lo | hi << 16;
-    }
-  }
-  return v;
 }
 
 // ---- dropout ----
@@ -196,11 +206,11 @@ __global__ __launch_bounds__(256) void dropout_counter_kernel(const T* __restric
     const int valid = n - i < 8 ? (int)(n - i) : 8;
     float f[8], r[8];
     if (valid == 8) {
-      load8<T, true>(x + i, 8, f);
-      if constexpr (RES) load8<T, true>(res + i, 8, r);
+      load8<T, true>(x + i, i, 8, f);
+      if constexpr (RES) load8<T, true>(res + i, i, 8, r);
     } else {
-      load8<T, false>(x + i, valid, f);
-      if constexpr (RES) load8<T, false>(res + i, valid, r);
+      load8<T, false>(x + i, i, valid, f);
+      if constexpr (RES) load8<T, false>(res + i, i, valid, r);
     }
     if (d.t != 0) drop8<true>(d, seed, offset, i, f);  // (0: evaluation, the residual's addition alone)
     if constexpr (RES)
@@ -295,12 +305,12 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_fwd_kernel(const T* __restr
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-      load8<T, VEC>(x + base + c, valid, f[j]);
+      load8<T, VEC>(x + base + c, c, valid, f[j]);
       if constexpr (DROP)
         if (valid > 0) drop8<VEC>(d, seed, offset, base + c, f[j]);
       if (res != nullptr) {
         float r[8];
-        load8<T, VEC>(res + base + c, valid, r);
+        load8<T, VEC>(res + base + c, c, valid, r);
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[j][k] += r[k];
       }
@@ -320,7 +330,7 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_fwd_kernel(const T* __restr
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
       if (w != nullptr) {
         float g[8];
-        load8<float, VEC>(w + c, valid, g);
+        load8<float, VEC>(w + c, c, valid, g);
 #pragma unroll
         for (int k = 0; k < 8; ++k) f[j][k] *= inv * g[k];
       } else {
@@ -368,7 +378,7 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restr
   float gw[GREG ? V : 1][8];
   auto weights = [&](int j, float* g) {
     const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-    if (w != nullptr) load8<float, VEC>(w + c, valid, g);
+    if (w != nullptr) load8<float, VEC>(w + c, c, valid, g);
     else
 #pragma unroll
       for (int k = 0; k < 8; ++k) g[k] = 1.f;
@@ -382,20 +392,23 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restr
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-      ra[j] = raw8<T, VEC>(dy + base + c, valid);
-      rb[j] = raw8<T, VEC>(h + base + c, valid);
+      ra[j] = raw8<T, VEC>(dy + base + c, c, valid);
+      rb[j] = raw8<T, VEC>(h + base + c, c, valid);
     }
     if (dh_out != nullptr) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
-        rc[j] = raw8<T, VEC>(dh_out + base + c, valid);
+        rc[j] = raw8<T, VEC>(dh_out + base + c, c, valid);
       }
     }
     const float inv = rstd[row];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      const int valid = min(max(N - (j * TPR + t) * 8, 0), 8);
+      settle8<T, VEC>(ra[j], valid);
+      settle8<T, VEC>(rb[j], valid);
       if constexpr (!GREG) weights(j, gw[0]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -412,6 +425,7 @@ __global__ __launch_bounds__(nthreads(TPR)) void rms_bwd_kernel(const T* __restr
     for (int j = 0; j < V; ++j) {
       const int c = (j * TPR + t) * 8, valid = N - c < 8 ? (N - c < 0 ? 0 : N - c) : 8;
       float o[8];
+      if (dh_out != nullptr) settle8<T, VEC>(rc[j], valid);
       if constexpr (!GREG) weights(j, gw[0]);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -502,10 +516,10 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
   for (long rr = r0; rr < r1; rr += 16) {
     const long r = rr + lr;
     float f[8];
-    load8<T, VEC>(x + r * N + c, r < r1 ? valid : 0, f);
+    load8<T, VEC>(x + r * N + c, c, r < r1 ? valid : 0, f);
     if constexpr (MASK) {
       float y[8];
-      load8<T, VEC>(ymask + r * N + c, r < r1 ? valid : 0, y);
+      load8<T, VEC>(ymask + r * N + c, c, r < r1 ? valid : 0, y);
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = y[k] <= 0.f ? 0.f : f[k];
     }
@@ -550,7 +564,7 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(const T* __restrict__ 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = blockIdx.y * 128 + i * 16 + lr;
-    load8<T, VEC>(w + (long)r * N + c, r < M ? valid : 0, f[i]);
+    load8<T, VEC>(w + (long)r * N + c, c, r < M ? valid : 0, f[i]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(f[i][k]));
   }
