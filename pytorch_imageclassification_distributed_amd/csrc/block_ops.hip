@@ -55,7 +55,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // four times as long as 16384 x 4096), and its last vector is cut.  In a 16-bit type that vector is the 8 elements that end
 // with the row, and settle8 shifts it down, zeros behind (a row shorter than 8 is read by elements): guarded loads of one
 // element follow each other, and a wait stands between each (16384 x 4095 bf16 norm, forward + backward: 144 + 220 us
-// against 124 + 137).  In float32 the shift costs more than they do (264 + 197 us against 239 + 168).
+// against 112 + 124).  In float32 the shift costs more than they do (264 + 197 us against 239 + 165).
 template <typename T, bool VEC>
 DEVI Raw8<T> raw8(const T* p, long c, int valid) {
   Raw8<T> v;
