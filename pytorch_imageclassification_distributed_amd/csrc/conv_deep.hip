@@ -1,22 +1,29 @@
-// Implicit-GEMM convolution (K1 forward / K2 data gradient) with prefetch depth 2: one wave per SIMD,
-// a 128 x 128 (or 128 x 64) output sub-tile per wave, two LDS buffers and two tiles of loads in flight.
+// Implicit-GEMM convolution (K1 forward / K2 data gradient) with prefetch depth 2: two LDS buffers and two tiles of
+// loads in flight.
 //
-// Why: on the compute-bound ResNet-50 GEMMs the 256 x 256 tile of conv_gemm_glds_kernel - 8 waves of 128 x 64, a
-// 2-buffer ring waited to vmcnt(0) every k-step, so ONE tile is in flight while one is computed - runs 945-1190 TF
-// where plain library GEMMs of the same sizes run 1313-1619 TF.  The layout follows from the LDS port: a wave's
-// (WTM + WTN) x 32 fragment reads feed WTM x WTN / 256 MFMAs, so 128 x 128 a wave reads a third less per MFMA than
-// 128 x 64; its accumulators are 128 * 128 / 64 = 256 registers a lane, which one wave per SIMD has to spare, and two
-// stages of (256 + 256) rows x 128 B are 128 KB of the 160 KB of LDS:
+// Why: the 256 x 256 tile of conv_gemm_glds_kernel waits for vmcnt(0) every k-step, so ONE tile is in flight while one
+// is computed; on the compute-bound ResNet-50 GEMMs it runs 945-1190 TF where plain library GEMMs of the same sizes run
+// 1313-1619 TF.  Here a tile has a step and a half to land:
 //
-//  * 4 waves in 2 x 2, each a (TM/2) x (BN/2) sub-tile: a 128 x 128 sub-tile issues one ds_read_b128 per
-//    4 MFMAs (the 8-wave 128 x 64 sub-tile: one per 2.7), so the LDS read port stays far from saturation;
-//    the accumulators live in AGPRs (256 of the 512 registers a lone wave owns);
 //  * a k-step reads BOTH 32-deep halves of its A / B fragments into registers; after the half-0 MFMAs
 //    every wave has its reads in registers, one barrier frees the buffer, and tile kt+2 is issued into
 //    it right there - it has until the middle of step kt+1 to land (~1.5 k-steps of MFMA time), where
 //    the 2-stage ring gives a load one k-step;
 //  * tile kt+1's half-0 fragments are read while the second half of step kt's MFMAs run, into the
-//    registers half 0 just released (two fragment sets in all, 128 VGPRs at 128 x 128);
+//    registers half 0 just released (two fragment sets in all, 96 VGPRs at 128 x 64 a wave);
+//  * 8 waves, two a SIMD: 128 x 64 a wave for 256 x 256 (2 x 4), 64 x 64 for 256 x 128 (4 x 2) and 512 x 64 (8 x 1), the
+//    accumulators (128 or 64 registers a lane) in AGPRs.  The split was taken by measurement with this schedule (grouped,
+//    spread variant; us of a bare GEMM M x N x K; one box, profiles/deep_conv_wave_layouts.txt):
+//      256 x 256 on               4096^3   8192^3   50176x512x2048   50176x2048x512   200704x1024x256
+//      8 waves, 2 x 4               99.3    743.5             99.6            129.3             200.2
+//      8 waves, 4 x 2               99.0    739.6             99.6            129.7             200.6
+//      4 waves, 2 x 2              100.1    732.5            104.4            150.0             232.4
+//      4 waves, 1 x 4              100.5    740.1            104.8            143.3             224.3
+//      4 waves, 4 x 1              100.9    737.8            104.9            148.7             229.9
+//      (one tile in flight, 2 x 4) 107.3    919.0            105.1            122.0             192.0
+//    Long sums do not tell the splits apart (the LDS port has room in all of them: a k-step reads 96 to 160 KB beside the
+//    64 KB that land, in the 2048 cycles of its MFMAs); with short ones the second wave of a SIMD hides the first loads
+//    and the outputs of the other;
 //  * the gather (LDS-DMA with per-lane im2col source offsets, zero padding = an out-of-range offset),
 //    the source-side XOR swizzle, the XCD-aware block remap and the fused epilogues are those of
 //    conv_gemm_glds_kernel (conv_common.h), so both kernels write identical tiles.
@@ -38,12 +45,11 @@ struct DeepCfg {
   static constexpr int MAIN = 2 * STAGE > EPI ? 2 * STAGE : EPI;
 };
 
-// The accumulators are pinned to AGPRs by an inline-asm MFMA ("+a"): with 256 accumulator registers the
-// compiler's own MFMA form fills the AGPR file exactly and its allocator then shuttles accumulators
-// through VGPRs (~400 v_accvgpr moves per 128 MFMAs).  hipcc pads no hazards around asm; the ones that
-// apply here are covered explicitly: SrcA/B come from ds_read (hipcc's lgkmcnt waits see asm operands),
-// each accumulator is re-used 64 MFMAs later, and s_nops separate the zero-init writes from the first
-// MFMA and the last MFMA from the epilogue's accumulator reads.
+// The accumulators are pinned to AGPRs by an inline-asm MFMA ("+a"): beside the fragments they take every register of a
+// wave, and with the compiler's own MFMA form its allocator shuttles them through VGPRs.  hipcc pads no hazards around
+// asm; the ones that apply here are covered explicitly: SrcA/B come from ds_read (hipcc's lgkmcnt waits see asm
+// operands), each accumulator is re-used a whole phase (4 MFMAs at least) later, and s_nops separate the
+// zero-init writes from the first MFMA and the last MFMA from the epilogue's accumulator reads.
 DEVI void mfma_acc(f32x4& acc, const bf16x8& a, const bf16x8& b) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b) : "memory");
 }
@@ -337,15 +343,15 @@ struct DeepEntry {
 };
 #define DEEP(TM, BN, WM, WN, V) {TM, BN, WM, WN, V, &launch_deep<TM, BN, WM, WN, V>}
 const DeepEntry g_deep[] = {
-    DEEP(256, 256, 2, 2, 0), DEEP(256, 256, 2, 2, 1), DEEP(256, 128, 2, 2, 0), DEEP(512, 64, 4, 1, 0),
+    DEEP(256, 256, 2, 4, 0), DEEP(256, 256, 2, 4, 1), DEEP(256, 128, 4, 2, 0), DEEP(512, 64, 8, 1, 0),
     // schedule variants of the 256 x 256 tile, and two diagnostics (variant & 6: wrong results, never tuned)
-    DEEP(256, 256, 2, 2, 8), DEEP(256, 256, 2, 2, 16), DEEP(256, 256, 2, 2, 32), DEEP(256, 256, 2, 2, 2),
-    DEEP(256, 256, 2, 2, 4),
+    DEEP(256, 256, 2, 4, 8), DEEP(256, 256, 2, 4, 16), DEEP(256, 256, 2, 4, 32), DEEP(256, 256, 2, 4, 2),
+    DEEP(256, 256, 2, 4, 4),
     // spread pieces + grouped tile order (4- / 8-row bands per XCD)
-    DEEP(256, 256, 2, 2, 16 | 64), DEEP(256, 256, 2, 2, 16 | 128), DEEP(256, 128, 2, 2, 16 | 64),
+    DEEP(256, 256, 2, 4, 16 | 64), DEEP(256, 256, 2, 4, 16 | 128), DEEP(256, 128, 4, 2, 16 | 64),
     // 32 x 32 x 16 MFMA blocks
-    DEEP(256, 256, 2, 2, 256), DEEP(256, 256, 2, 2, 16 | 64 | 256), DEEP(256, 128, 2, 2, 16 | 64 | 256),
-    DEEP(256, 256, 2, 2, 1 | 256),
+    DEEP(256, 256, 2, 4, 256), DEEP(256, 256, 2, 4, 16 | 64 | 256), DEEP(256, 128, 4, 2, 16 | 64 | 256),
+    DEEP(256, 256, 2, 4, 1 | 256),
 };
 #undef DEEP
 

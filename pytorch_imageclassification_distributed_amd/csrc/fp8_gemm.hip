@@ -292,6 +292,9 @@ __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
 //   second half (B 2, 3):            the 16 LDS-DMA pieces of tile kt + 2 go into this buffer, one an MFMA (two an MFMA
 //                                    stall at the 64 B a cycle of the load path: 206 us against 186), and B 0, 1 and,
 //                                    block by block, A of kt + 1 are read from the other one.
+// 256 x 256 with the ring kernel's schedule, same size: 8 waves of 64 x 128 313 us, of 128 x 64 342, 4 of 128 x 128 482 (it
+// spills there: the builtin's accumulators and the fragments share the file), 128 x 128 tiles 405; this schedule needs the
+// registers that only a lone wave of a SIMD has.
 // 8192 x 8192 x 4096: 211 us (2.6 PFLOP/s), 186 of it the main loop; with loads that always hit L2, or a prefetch into
 // L2, no faster; without any load 170 (the clock under full load), so the matrix pipe bounds it.  The rest is the
 // epilogue and a block's first loads; persistent blocks that issue the next tile's loads before the outputs were slower

@@ -3,7 +3,8 @@
 // Both operands are row-major with the contracted index outermost, so their MFMA fragments are read from LDS images
 // [64 rows][256 columns] by transposing reads.  256 x 256 outputs on 4 waves of 128 x 128, one block a CU, 32 x 32 x 16
 // instructions; a stage of 64 rows is 64 MFMAs of 32 cycles a wave, fed by 64 ds_read_b64_tr_b16 and 16 LDS-DMA pieces:
-// the bytes and cycles of the 8-bit product's large tile, and its schedule - one barrier a stage, fragments refilled in
+// the bytes and cycles of the 8-bit product's large tile (128 KB read and 64 KB written through the LDS port in the 2048
+// cycles of a stage's MFMAs; waves of 128 x 64 would read 192 KB), and its schedule - one barrier a stage, fragments refilled in
 // the registers whose last MFMA has been issued, memory instructions one by one between the MFMAs:
 //   first half of a stage (B blocks 0, 1):  B 2, 3 are read;
 //   middle: the next stage has landed, this buffer's reads have ended in every wave: the barrier;

@@ -7,8 +7,15 @@
 // for the one stage in flight at every barrier, and each k-step starts with its fragment reads' latency
 // exposed, since every wave reaches the barrier together.  Here, as in conv_deep_kernel:
 //
-//  * 4 waves in 2 x 2, each a (WBM/2) x (TN/2) sub-tile - at 256 x 256, 128 x 128 per wave, accumulators
-//    pinned in AGPRs by inline-asm MFMAs;
+//  * 128 x 256 and 256 x 128 on 8 waves of 64 x 64, 256 x 256 on 4 waves of 128 x 128, accumulators pinned in AGPRs by
+//    inline-asm MFMAs.  Measured both ways (profiles/deep_conv_wave_layouts.txt; us, ResNet-50 batch 1024):
+//                                  128 x 256        256 x 128        256 x 256
+//                                  4 waves    8     4 waves    8     4 waves    8
+//      256 -> 256, 3x3, 14 x 14        429  353         426  370         302  520
+//      1024 -> 256, 1x1, 14 x 14       196  174         192  181         153  282
+//      2048 -> 512, 1x1, 7 x 7         196  168         181  166         146  261
+//    (at 256 x 256 the fragments and the gather's state pass the 128 VGPRs of a wave beside 128 accumulators: its loop
+//    spills);
 //  * two LDS stages of 64 pixels, two stages of LDS-DMA in flight: after phase A (the half-0 MFMAs, with the
 //    half-1 fragment reads spread among them) one barrier frees the stage and stage kt+2 is issued into it;
 //  * the next stage's half-0 fragments are read during the second half of this stage's half-1 MFMAs.
@@ -19,10 +26,10 @@
 // carries), the split-K slab / atomic epilogue and the XCD-aware tile order are that kernel's too.
 // Scope: plain dY and X (no fused BN-backward / BN-apply operand form).
 //
-// Measured (profiles/r10p_wgrad_deep_ab.txt): numerically exact, but 5-18 % slower than the 8-wave
-// 256 x 256 conv_wgrad_glds_kernel (stages 7) on the ResNet-50 shapes - e.g. 256-ch 3x3 at 14 x 14: 301 vs
-// 255 us - so the tuner, which times it as a candidate, keeps picking stages 7 / 1 there.  The transposed
-// fragments cost two LDS instructions each, and one wave per SIMD cannot hide what the two waves of the
+// Measured: numerically exact, but 5-20 % slower than the 8-wave 256 x 256 conv_wgrad_glds_kernel (stages 7) on the
+// ResNet-50 shapes - e.g. 256-ch 3x3 at 14 x 14: 302 vs 246 us - so the tuner, which times it as a candidate, keeps
+// picking stages 7 / 1 there; 512-ch 3x3 at 7 x 7 comes nearest (256 x 128: 338 vs 348 us, stages 1 293).  The
+// transposed fragments cost two LDS instructions each, and one wave per SIMD cannot hide what the two waves of the
 // 8-wave kernel hide for each other.
 #include "conv_common.h"
 
@@ -59,7 +66,8 @@ DEVI int wd_fdiv(int n, int d, float inv, int& rem) {
 
 template <int WBM, int TN>
 struct WdCfg {
-  static constexpr int NW = 4, NTH = 256, WM = 2, WN = 2;
+  static constexpr int NW = WBM == 256 && TN == 256 ? 4 : 8, NTH = 64 * NW;
+  static constexpr int WN = NW == 8 && TN == 256 ? 4 : 2, WM = NW / WN;
   static constexpr int AROWB = WBM * 2, BROWB = TN * 2;
   static constexpr int A_BYTES = DW_KPS * AROWB, STAGE = A_BYTES + DW_KPS * BROWB;
   static constexpr int LDT = TN + 4;                 // floats per staged epilogue row
@@ -68,7 +76,7 @@ struct WdCfg {
 };
 
 template <int WBM, int TN>
-__global__ __launch_bounds__(256, 1) void wgrad_deep_kernel(const WgradParams p) {
+__global__ __launch_bounds__((WdCfg<WBM, TN>::NTH), 1) void wgrad_deep_kernel(const WgradParams p) {
   using Cfg = WdCfg<WBM, TN>;
   constexpr int NW = Cfg::NW, NTH = Cfg::NTH, WN = Cfg::WN, WM = Cfg::WM;
   constexpr int AROWB = Cfg::AROWB, BROWB = Cfg::BROWB;
@@ -289,7 +297,7 @@ __global__ __launch_bounds__(256, 1) void wgrad_deep_kernel(const WgradParams p)
 template <int WBM, int TN>
 void launch_wd(const WgradParams& p, int splits, hipStream_t stream) {
   const dim3 grid(cdiv(p.Cout, WBM) * cdiv(p.Ntot, TN), splits);
-  hipLaunchKernelGGL((wgrad_deep_kernel<WBM, TN>), grid, dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((wgrad_deep_kernel<WBM, TN>), grid, dim3(WdCfg<WBM, TN>::NTH), 0, stream, p);
 }
 
 }  // namespace
