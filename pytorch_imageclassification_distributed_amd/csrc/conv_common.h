@@ -437,6 +437,30 @@ DEVI void wait_vmcnt_lds() {
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (((N >> 4) & 3) << 14));
 }
 
+// Accumulators that inline-asm MFMAs keep in AGPRs: hipcc knows nothing of those instructions' hazards, and an s_nop
+// without operands orders nothing but other volatile asm - hipcc may move the writes that zero the accumulators behind
+// it, or the reads of the results before it.  So every accumulator passes through an operand on the wait's near side.
+template <typename A, int R, int C>
+DEVI void pin_acc(A (&acc)[R][C]) {
+  static_assert(C % 2 == 0, "two blocks a statement");
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < C; j += 2) asm volatile("" : "+a"(acc[i][j]), "+a"(acc[i][j + 1]));
+}
+// zeroed accumulators -> the first MFMA
+template <typename A, int R, int C>
+DEVI void acc_ready(A (&acc)[R][C]) {
+  pin_acc(acc);
+  asm volatile("s_nop 7" ::: "memory");
+}
+// the last MFMAs (16 passes at most) -> the first read of an accumulator
+template <typename A, int R, int C>
+DEVI void acc_done(A (&acc)[R][C]) {
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  pin_acc(acc);
+}
+
 DEVI void glds16(const void* src, char* lds_wave_base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }

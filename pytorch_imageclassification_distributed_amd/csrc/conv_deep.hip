@@ -48,7 +48,7 @@ struct DeepCfg {
 // The accumulators are pinned to AGPRs by an inline-asm MFMA ("+a"): beside the fragments they take every register of a
 // wave, and with the compiler's own MFMA form its allocator shuttles them through VGPRs.  hipcc pads no hazards around
 // asm; the ones that apply here are covered explicitly: SrcA/B come from ds_read (hipcc's lgkmcnt waits see asm
-// operands), each accumulator is re-used a whole phase (4 MFMAs at least) later, and s_nops separate the
+// operands), each accumulator is re-used a whole phase (4 MFMAs at least) later, and acc_ready / acc_done separate the
 // zero-init writes from the first MFMA and the last MFMA from the epilogue's accumulator reads.
 DEVI void mfma_acc(f32x4& acc, const bf16x8& a, const bf16x8& b) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b) : "memory");
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void conv_deep_kernel(const ConvPa
   for (int i = 0; i < AR; ++i)
 #pragma unroll
     for (int j = 0; j < AC; ++j) acc[i][j] = AccT{};
-  asm volatile("s_nop 7");
+  acc_ready(acc);
 
   const int nk = (p.K + BK - 1) / BK;
   const int fr = lane & 15, fq = lane >> 4;
@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void conv_deep_kernel(const ConvPa
     if constexpr (SETPRIO) __builtin_amdgcn_s_setprio(0);
   }
   wait_vmcnt<0>();  // the zero pieces of the last two steps land before the epilogue reuses the ring
-  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15");  // last MFMA -> accumulator reads
+  acc_done(acc);
   __syncthreads();
   // the accumulators (AGPRs) -> the bf16 tile in LDS, one 16-row fragment row at a time: left to itself
   // the scheduler reads every AGPR out before the first store and spills

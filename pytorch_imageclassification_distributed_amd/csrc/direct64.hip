@@ -246,7 +246,7 @@ __global__ __launch_bounds__(256, 1) void direct64_kernel(const D64Args a) {
     }
     // these accumulators are read by VALU in the next step's epilogue: MFMA -> VALU read hazard cover (the
     // compiler does not see through the asm)
-    asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+    acc_done(acc[PAR]);
     prev = t;
     t += tstride;
     buf ^= 1;

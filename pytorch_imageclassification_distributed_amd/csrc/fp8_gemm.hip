@@ -433,7 +433,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x16_t{};
-  asm volatile("s_nop 7");
+  acc_ready(acc);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     a[i][0] = frag(buf0, oa, i, 0);
@@ -462,10 +462,7 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
     step(std::integral_constant<int, 1>{}, kt + 1);
     kt += 2;
   } while (kt < nk);
-  // the last MFMAs' results before the first read of an accumulator: waits that every accumulator depends on
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]));
+  acc_done(acc);
   wait_vmcnt<0>();  // (LDS-DMA must not outlive the block)
   const int cm = m0 + wm * 128, cn = n0 + wn * 128;
   const bool vec = (p.ldc & 7) == 0;  // then a lane's 8 columns are all inside or all outside

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x16_t{};
-  asm volatile("s_nop 7");
+  acc_ready(acc);
 
   bf16x8 a[4][4], b[4][4];
 #pragma unroll
@@ -182,10 +182,7 @@ __global__ __launch_bounds__(256, 1) void rows_grad_kernel(const RowsGrad p) {
     stage(std::integral_constant<int, 1>{}, st + 1);
     st += 2;
   } while (st < stages);
-  // the last MFMAs' results before the first read of an accumulator: waits that every accumulator depends on
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][0]), "+a"(acc[i][1]), "+a"(acc[i][2]), "+a"(acc[i][3]));
+  acc_done(acc);
   wait_vmcnt<0>();  // (LDS-DMA must not outlive the block)
 
   const int cn = n0 + wm * 128, ck = k0 + wn * 128;

@@ -180,7 +180,7 @@ __global__ __launch_bounds__((WdCfg<WBM, TN>::NTH), 1) void wgrad_deep_kernel(co
   for (int i = 0; i < RM; ++i)
 #pragma unroll
     for (int j = 0; j < RN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  asm volatile("s_nop 7");
+  acc_ready(acc);
 
   // fragment q of k-half h from stage buffer buf (A blocks first, then B): permuted k order, identical for
   // A and B - elements 0-3 <- pixel rows 4g + tq, elements 4-7 <- rows 16 + 4g + tq
@@ -251,7 +251,7 @@ __global__ __launch_bounds__((WdCfg<WBM, TN>::NTH), 1) void wgrad_deep_kernel(co
     }
   }
   wait_vmcnt<0>();  // the two stages past the end land before the epilogue reuses the ring
-  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15");  // last MFMA -> accumulator reads
+  acc_done(acc);
   __syncthreads();
 
   // acc[i][j][r] = dW[co0 + wm*WTM + i*16 + fr][j0 + wn*WTN + j*16 + fq*4 + r]; the fp32 tile is staged
