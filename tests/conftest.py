@@ -44,6 +44,20 @@ def pytest_collection_modifyitems(config, items):
             it.add_marker(skip)
 
 
+# Tests that compare two paths of one block elementwise behind ReLUs.  With kernels picked by timing the two paths may add
+# batch-norm statistics in different orders, and an element within a rounding of zero then changes sides of the ReLU: the
+# weight gradient moves by 12 % of its largest entry (test_inception_heads_oracle.py compares each path with 64 bits under
+# any choice of kernels).  Both paths take their kernels from the shape here, so that what differs is the path alone.
+_SAME_KERNELS = {"test_inception_sibling_heads_merged"}
+
+
+@pytest.fixture(autouse=True)
+def _kernels_by_shape(request, monkeypatch):
+    if getattr(request.node, "originalname", None) in _SAME_KERNELS:
+        from pytorch_imageclassification_distributed_amd.ops._hip import gemm
+        monkeypatch.setattr(gemm, "CONV_STAGES", "0")
+
+
 @pytest.fixture(autouse=True)
 def _bounds_record():
     """With the bounds-checked library (IMGCLS_EXT=_C_bounds.so, built by build.py with IMGCLS_BOUNDS_CHECK; csrc/
