@@ -5,6 +5,7 @@
 // The autograd nodes are C++: a small call is bound by the host, and a Python node costs it twice the time of one of
 // torch's own (4 x 2048 dropout, forward and backward: 70 us with a Python node, 46 us for torch's product).
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -245,6 +246,15 @@ bool has(const OT& t) { return t.has_value() && t->defined(); }
 Tensor or_undefined(const OT& t) { return has(t) ? *t : Tensor(); }
 bool wants(const OT& t) { return has(t) && t->requires_grad(); }
 
+// The operators have no forward-mode derivative.  Their nodes refuse one, but a dual tensor need not ask for a gradient
+// (and may come under no_grad), and then no node is made: without this the tangent would be lost without an error.
+void no_tangent(const char* what, std::initializer_list<Tensor> in) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor& t : in)
+    TORCH_CHECK_NOT_IMPLEMENTED(!(t.defined() && t._fw_grad(/*level=*/0).defined()), what,
+                                " has no forward-mode derivative, and an input carries a tangent");
+}
+
 Tensor fresh(at::IntArrayRef size, const Tensor& like, at::ScalarType st) { return at::empty(size, like.options().dtype(st)); }
 
 struct Blocks {
@@ -333,6 +343,7 @@ struct DropoutCounterNode : torch::autograd::Function<DropoutCounterNode> {
 };
 
 Tensor op_dropout_counter(const Tensor& x, const OT& residual, const OT& state, uint64_t seed, uint64_t offset, int64_t t) {
+  no_tangent("dropout_counter", {x, or_undefined(residual)});
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual)))  // nothing asks for a gradient
     return drop_forward(x, residual, state, {t, seed, offset});
   return DropoutCounterNode::apply(x, residual, state, t, (int64_t)seed, (int64_t)offset);
@@ -402,6 +413,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
 // [y] or [y, h]
 std::vector<Tensor> op_rms_norm(const Tensor& x, const OT& residual, const OT& weight, const OT& state, uint64_t seed,
                                 uint64_t offset, int64_t t, double eps, py::object slot) {
+  no_tangent("rms_norm", {x, or_undefined(residual), or_undefined(weight)});
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || wants(residual) || wants(weight))) {
     RmsOut o = rms_forward(dense16(x), residual, weight, state, {t, seed, offset}, eps, false);
     if (has(residual)) return {o.y, o.h};
@@ -593,6 +605,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
 
 Tensor op_linear_fp8(const Tensor& x, const Tensor& weight, const OT& bias, int64_t act, py::object wslot,
                      py::object bslot) {
+  no_tangent("linear_fp8", {x, weight, or_undefined(bias)});
   const bool grad = at::GradMode::is_enabled(), nx = grad && x.requires_grad(), nw = grad && weight.requires_grad();
   if (!(nx || nw || (grad && wants(bias)))) return linear_forward(dense16(x.detach()), weight, bias, act, false, false).y;
   return LinearFp8Node::apply(x, weight, bias, act, nx, nw, slot_value(wslot), slot_value(bslot));

@@ -23,6 +23,7 @@ import os
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .fp8_blocks import (FLOATS, Fp8Blocks, dequantize_ref, drop_ref, drop_threshold, linear_fp8_ref, quantize_rows_ref,
                          quantize_tiles_ref, rms_norm_fp8_ref, rms_norm_ref)
@@ -272,7 +273,8 @@ def dropout_counter(x, p, training=True, seed=None, offset=0, residual=None):
     graph sees the values it holds at each replay; changing it between forward and backward is an error); or None, which
     draws both from the device's generator.  Every (seed, offset) pair is an independent mask over up to 2^67 elements.
     ``p`` is rounded to a multiple of 2^-16; the kept values are scaled by 1 / (1 - that).  Elements are numbered in
-    row-major order whatever the strides; the result is row-major.  A dropped infinity or NaN leaves 0.
+    row-major order whatever the strides; the result is row-major.  A dropped infinity or NaN leaves 0.  Differentiable
+    once, in reverse mode (a forward-mode tangent is refused on the GPU).
     """
     _check_floats("dropout_counter", x)
     _check_like("dropout_counter", "residual", residual, x)
@@ -334,7 +336,14 @@ def rms_norm_fp8(x, norm, residual=None):
     return out if residual is None else (out, h)
 
 
+def _refuse_tangent(name, *tensors):
+    if forward_ad._current_level >= 0 and forward_ad._is_fwd_grad_enabled() and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative, and an input carries a tangent")
+
+
 def _refuse_grad(name, *tensors):
+    _refuse_tangent(name, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or train through linear_fp8")
 
@@ -354,6 +363,7 @@ def quantize_fp8_weight(w):
     _check_floats("quantize_fp8_weight", w)
     if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1:
         raise ValueError(f"quantize_fp8_weight: a weight is [N, K], got {tuple(w.shape)}")
+    _refuse_tangent("quantize_fp8_weight", w)
     w = w.detach()
     return _hip().quantize_fp8_weight(w) if use_hip(w) else quantize_tiles_ref(w)
 

@@ -1,0 +1,72 @@
+"""What the documentation of the pre-norm 8-bit linear block (ops/functional.py dropout_counter, rms_norm, rms_norm_fp8,
+quantize_fp8, matmul_fp8, linear_fp8) allows or refuses beyond plain calls: forward-mode tangents, operands that a user
+lays out, unusual sizes, calls from several threads."""
+import pytest
+import torch
+import torch.nn as nn
+from torch.autograd import forward_ad
+
+from pytorch_imageclassification_distributed_amd.ops import functional as Fx
+from pytorch_imageclassification_distributed_amd.ops import fp8_blocks as fb
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+gpu = pytest.mark.gpu
+
+
+def rand(shape, t, dev, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(t).to(dev)
+
+
+# ---------------------------------------------------------------------------
+# forward mode
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_tangent_is_never_lost(dev, grad):
+    """An operator hands a tangent on or raises; it does not return a result without one."""
+    x = rand((4, 64), torch.float32, dev, 1)
+    frozen = nn.RMSNorm(64).to(dev).requires_grad_(False), nn.Linear(64, 8).to(dev).requires_grad_(False)
+    ones = torch.ones_like(x)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        d = forward_ad.make_dual(x, ones)
+        w = forward_ad.make_dual(frozen[1].weight.detach(), torch.ones_like(frozen[1].weight))
+        dual_norm, dual_lin = nn.RMSNorm(64).to(dev).requires_grad_(False), nn.Linear(64, 8).to(dev).requires_grad_(False)
+        del dual_norm.weight, dual_lin.weight
+        dual_norm.weight, dual_lin.weight = d[0], w
+        q, qw = Fx.quantize_fp8(x), Fx.quantize_fp8_weight(frozen[1].weight)
+        calls = [lambda: Fx.rms_norm(d, frozen[0]), lambda: Fx.rms_norm(x, frozen[0], residual=d), lambda: Fx.rms_norm(x, dual_norm),
+                 lambda: Fx.rms_norm(x, frozen[0], residual=d, p=0.5, seed=1),
+                 lambda: Fx.linear_fp8(d, frozen[1]), lambda: Fx.linear_fp8(x, dual_lin, "relu"),
+                 lambda: Fx.quantize_fp8(d), lambda: Fx.quantize_fp8_weight(w), lambda: Fx.rms_norm_fp8(d, frozen[0]),
+                 lambda: Fx.rms_norm_fp8(x, frozen[0], residual=d), lambda: Fx.matmul_fp8(q, qw, bias=w[:, 0])]
+        for i, f in enumerate(calls):
+            with pytest.raises(NotImplementedError):
+                f()
+        for kw in (dict(x=d), dict(x=d, residual=d), dict(x=x, residual=d), dict(x=x, residual=d, training=False)):
+            if dev == "cuda":
+                with pytest.raises(NotImplementedError, match="tangent"):
+                    Fx.dropout_counter(p=0.5, seed=3, **kw)
+            else:
+                y = Fx.dropout_counter(p=0.5, seed=3, **kw)
+                want = torch.zeros_like(x)
+                if kw["x"] is d:
+                    want = want + Fx.dropout_counter(ones, 0.5, seed=3)
+                if kw.get("residual") is not None:
+                    want = want + 1
+                assert torch.equal(forward_ad.unpack_dual(y).tangent, want)
+        # without a tangent, or with forward gradients switched off, nothing is refused
+        assert Fx.rms_norm(x, frozen[0]).shape == x.shape and Fx.linear_fp8(x, frozen[1]).shape == (4, 8)
+        with forward_ad._set_fwd_grad_enabled(False):
+            assert Fx.linear_fp8(d, frozen[1]).shape == (4, 8) and Fx.quantize_fp8(d).shape == (4, 64)
+
+
+@gpu
+def test_function_transforms_are_refused():
+    x = rand((4, 64), torch.float32, "cuda", 2)
+    norm, lin = nn.RMSNorm(64).cuda().requires_grad_(False), nn.Linear(64, 8).cuda().requires_grad_(False)
+    for f in (lambda v: Fx.dropout_counter(v, 0.5, seed=1), lambda v: Fx.rms_norm(v, norm), lambda v: Fx.linear_fp8(v, lin)):
+        with pytest.raises(Exception):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+        with pytest.raises(Exception):
+            torch.vmap(f)(x.view(4, 1, 64))
