@@ -38,7 +38,7 @@ int rows_grad_plan(int, int, int, int, int*);
 int rows_grad_launch(const bf16_t*, const bf16_t*, float*, float*, int, int, int, int, int, int, int, hipStream_t);
 void fp8_gemm_force(int);
 int fp8_gemm_launch(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, const float*, int, int, int,
-                    long, long, int, int, int, long, int, int, hipStream_t);
+                    int, long, long, int, int, int, long, int, int, hipStream_t);
 
 namespace {
 
@@ -219,7 +219,7 @@ void fp8_gemm(Tensor a, Tensor as, Tensor b, Tensor bs, Tensor c, OT bias, int64
   TORCH_CHECK(((M + 15) / 16) * ((N + 15) / 16) < (1LL << 31), "matmul_fp8: grid too large");
   ok(fp8_gemm_launch((const uint8_t*)a.data_ptr(), as.data_ptr<uint8_t>(), (const uint8_t*)b.data_ptr(),
                      bs.data_ptr<uint8_t>(), c.data_ptr(), (const float*)raw(bias), (int)M, (int)N, (int)(a.size(1) / 128),
-                     a.size(1), b.size(1), (int)as.size(1), (int)bs.size(1), btile == 128 ? 7 : 0, N, act, code,
+                     (int)(K % 128), a.size(1), b.size(1), (int)as.size(1), (int)bs.size(1), btile == 128 ? 7 : 0, N, act, code,
                      stream_of(a)),
      "matmul_fp8");
 }
@@ -526,8 +526,8 @@ LinearOut linear_forward(const Tensor& x, const Tensor& weight, const OT& bias, 
   }
   ok(quant_tiles_launch(w.data_ptr(), p + bq, p + bs, t, ts, (int)n, (int)k, kp, (int)ks, np, (int)ns, tw, st), "linear_fp8");
   o.y = fresh({m, n}, x, x.scalar_type());
-  ok(fp8_gemm_launch(p + aq, p + as, p + bq, p + bs, o.y.data_ptr(), (const float*)raw(b), (int)m, (int)n, (int)blocks_of(k), kp,
-                     kp, (int)ks, (int)ks, 7, n, (int)act, tx, st),
+  ok(fp8_gemm_launch(p + aq, p + as, p + bq, p + bs, o.y.data_ptr(), (const float*)raw(b), (int)m, (int)n, (int)blocks_of(k), 0,
+                     kp, kp, (int)ks, (int)ks, 7, n, (int)act, tx, st),
      "linear_fp8");
   return o;
 }
@@ -581,8 +581,8 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
       Layout lt;
       const int64_t t = lt.add(k * np), ts = lt.add(blocks_of(k) * ns);
       uint8_t* w = wt.data_ptr<uint8_t>();
-      ok(fp8_gemm_launch(p + q, p + sc, w + t, w + ts, dx.data_ptr(), nullptr, (int)m, (int)k, (int)blocks_of(n), np, np, (int)ns,
-                         (int)ns, 7, k, 0, type, st),
+      ok(fp8_gemm_launch(p + q, p + sc, w + t, w + ts, dx.data_ptr(), nullptr, (int)m, (int)k, (int)blocks_of(n), 0, np, np,
+                         (int)ns, (int)ns, 7, k, 0, type, st),
          "linear_fp8 backward");
     }
     if (nw) {

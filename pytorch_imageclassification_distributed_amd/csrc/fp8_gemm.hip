@@ -18,6 +18,7 @@ struct Fp8Gemm {
   const uint8_t* A; const uint8_t* As; const uint8_t* B; const uint8_t* Bs;
   void* C; const float* bias;
   int M, N, nk;      // nk = blocks of 128 columns
+  int tail;          // columns of the last block where it is not whole and the bytes behind them may be anything; else 0
   long lda, ldb;     // bytes a row
   int ldsa, ldsb;    // scale bytes a scale row (multiples of 4)
   int bshift;        // log2 of the B rows that share a scale row: 0 or 7
@@ -73,6 +74,29 @@ DEVI void store4(const Fp8Gemm& p, int m, int n, const f32x4& v, const float* bi
   }
 }
 
+// Bytes behind the last column count as zeros, whatever they are (times another operand's zero a NaN byte would still
+// make the sum NaN).  bytes[4 i, 4 i + 4) of a piece whose first `keep` bytes are inside:
+DEVI uint32_t inside(int keep, int i) {
+  const int b = keep - 4 * i;
+  return b >= 4 ? ~0u : b <= 0 ? 0u : (1u << (8 * b)) - 1;
+}
+// A stage of LDS, ROWS x 128 B: every wave sees the last block's tile landed when it calls this, and cleared when it
+// returns.  (In LDS, between a barrier and the fragments' reads: once a launch, and nothing added to the other steps.)
+template <int ROWS, int NT>
+DEVI void clear_tail(char* stage, int tail) {
+  const int part = tail >> 4, keep = tail & 15;  // chunk `part` of a row is the first that is not whole
+  for (int row = threadIdx.x; row < ROWS; row += NT) {
+    uint4* const at = (uint4*)(stage + swz(row, part));
+    uint4 v = *at;
+    v.x &= inside(keep, 0); v.y &= inside(keep, 1); v.z &= inside(keep, 2); v.w &= inside(keep, 3);
+    *at = v;
+#pragma unroll
+    for (int ch = 1; ch < 8; ++ch)
+      if (ch > part) *(uint4*)(stage + swz(row, ch)) = make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+}
+
 DEVI void bias4(const Fp8Gemm& p, int n, float* b) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) b[r] = p.bias != nullptr && n + r < p.N ? p.bias[n + r] : 0.f;
@@ -116,7 +140,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
     const int row = wid * (BN / NW) + i * 8 + lrow;
     vb[i] = (unsigned)(row * (int)p.ldb + (pch ^ ((row >> 1) & 7)) * 16);
   }
-  const int nk = p.nk;
+  const int nk = p.nk, tail_step = p.tail ? nk - 1 : -1;
   // every step issues its pieces (past the last tile from an empty resource), so the counted waits are constant
   auto issue = [&](int kt, char* buf) __attribute__((always_inline)) {
     const bool live = kt < nk;
@@ -157,10 +181,12 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
 
   // step kt = S n + U: tile kt has landed (S - 2 younger ones are in flight), every wave has left step kt - 1, whose
   // stage takes tile kt + S - 1
-  auto step = [&](auto c, int kt) __attribute__((always_inline)) {
+  auto step = [&](auto c, int kt, auto last) __attribute__((always_inline)) {
     constexpr int U = decltype(c)::value;
     wait_vmcnt_lds<(S - 2) * LPS>();
     __builtin_amdgcn_s_barrier();
+    if constexpr (decltype(last)::value)
+      if (kt == tail_step) clear_tail<BM + BN, 64 * NW>(stage(c), p.tail);
     issue(kt + S - 1, stage(std::integral_constant<int, U + S - 1>{}));
     if (S == 4 ? U == 0 : (kt & 3) == 0) {
       const int nxt = min((kt >> 2) + 1, (nk - 1) >> 2);
@@ -198,24 +224,29 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
     issue(1, s1);
     issue(2, s2);
   }
-  // (whole rounds of the ring, then the rest: with exits inside the loop hipcc joins their states at its head, and waits
-  // for every load there)
+  // (whole rounds of the ring, then the rest, a cut last step always in it: with exits inside the loop hipcc joins their
+  // states at its head, and waits for every load there; a branch there costs it half its registers again)
+  const int whole = nk - (p.tail ? 1 : 0);
+  constexpr std::false_type N{};
+  constexpr std::true_type Y{};
   int kt = 0;
-  for (; kt + S <= nk; kt += S) {
-    step(std::integral_constant<int, 0>{}, kt);
-    step(std::integral_constant<int, 1>{}, kt + 1);
+  for (; kt + S <= whole; kt += S) {
+    step(std::integral_constant<int, 0>{}, kt, N);
+    step(std::integral_constant<int, 1>{}, kt + 1, N);
     if constexpr (S == 4) {
-      step(std::integral_constant<int, 2>{}, kt + 2);
-      step(std::integral_constant<int, 3>{}, kt + 3);
+      step(std::integral_constant<int, 2>{}, kt + 2, N);
+      step(std::integral_constant<int, 3>{}, kt + 3, N);
     }
   }
   if (kt < nk) {
-    step(std::integral_constant<int, 0>{}, kt);
-    if constexpr (S == 4) {
-      if (kt + 1 < nk) {
-        step(std::integral_constant<int, 1>{}, kt + 1);
-        if (kt + 2 < nk) step(std::integral_constant<int, 2>{}, kt + 2);
-      }
+    step(std::integral_constant<int, 0>{}, kt, Y);
+    if (kt + 1 < nk) {
+      step(std::integral_constant<int, 1>{}, kt + 1, Y);
+      if constexpr (S == 4)
+        if (kt + 2 < nk) {
+          step(std::integral_constant<int, 2>{}, kt + 2, Y);
+          if (kt + 3 < nk) step(std::integral_constant<int, 3>{}, kt + 3, Y);
+        }
     }
   }
   wait_vmcnt<0>();
@@ -234,7 +265,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_gemm_kernel(const Fp8Gemm p)
 // 16 RM rows x 16 columns a block, its 8 waves each a share of the k-steps, their partial sums joined through LDS in a
 // fixed order.  The weights' bytes bound it, so they go from memory straight into the fragments (16 rows x 128 whole
 // bytes a wave and k-step; no LDS, no barrier before the join), and a launch has N / 16 x 8 waves to keep them coming.
-template <int RM, int ACT, int CT>
+// CUT: the last block is not whole (as a test of p.tail it cost the other case 3 %, and 1 % in the large tile)
+template <int RM, bool CUT, int ACT, int CT>
 __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
   constexpr int W = 8;
   __shared__ f32x4 part[W][RM][64];
@@ -256,8 +288,9 @@ __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
   f32x4 acc[RM];
 #pragma unroll
   for (int i = 0; i < RM; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  const bool cut = CUT && wid == W - 1;  // this wave has the last block
 #pragma unroll 4
-  for (int kt = k0; kt < k1; ++kt) {
+  for (int kt = k0; kt < k1 - (cut ? 1 : 0); ++kt) {
     const uint8_t* b = B + (long)kt * 128;
     const i32x8 wb = frag8((const char*)b, (const char*)b + 64);
     const int sw = Bs[kt];
@@ -267,6 +300,22 @@ __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
       const i32x8 xa = frag8((const char*)a, (const char*)a + 64);
       acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wb, xa, acc[i], 0, 0, 0, sw, 0, (int)As[i][kt]);
     }
+  }
+  if (cut) {
+    const long at = (long)(nk - 1) * 128;
+    i32x8 tb = frag8((const char*)B + at, (const char*)B + at + 64), ta[RM];
+#pragma unroll
+    for (int i = 0; i < RM; ++i) ta[i] = frag8((const char*)A[i] + at, (const char*)A[i] + at + 64);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const int m = (int)inside(p.tail - fq * 16 - (d >> 2) * 64, d & 3);
+      tb[d] &= m;
+#pragma unroll
+      for (int i = 0; i < RM; ++i) ta[i][d] &= m;
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+      acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(tb, ta[i], acc[i], 0, 0, 0, (int)Bs[nk - 1], 0, (int)As[i][nk - 1]);
   }
 #pragma unroll
   for (int i = 0; i < RM; ++i) part[wid][i][lane] = acc[i];
@@ -316,7 +365,7 @@ DEVI void mma32(f32x16_t& acc, const i32x8& b, const i32x8& a, uint32_t sb, uint
 constexpr int BIG_STAGE = 512 * 128;
 constexpr int BIG_BAND = 4;     // tile rows of a band
 
-template <int ACT, int CT>
+template <bool CUT, int ACT, int CT>
 __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
   // separate arrays, not one: hipcc makes an LDS read wait for every LDS-DMA that may write what it reads, and tells
   // them apart by the array alone
@@ -404,6 +453,8 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
     wait_vmcnt<0>();
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
+    if constexpr (CUT)
+      if (kt + 2 == nk) clear_tail<512, 256>(nxt(), p.tail);
     if constexpr (P == 0) {
       if ((kt & 2) == 0) scales(min((kt >> 2) + 1, words - 1));
     } else {
@@ -429,6 +480,8 @@ __global__ __launch_bounds__(256, 1) void fp8_gemm_big_kernel(const Fp8Gemm p) {
   scales(0);
   wait_vmcnt<0>();
   __builtin_amdgcn_s_barrier();
+  if constexpr (CUT)
+    if (nk == 1) clear_tail<512, 256>(buf0, p.tail);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -538,7 +591,9 @@ void launch_tile(const Fp8Gemm& p, hipStream_t s) {
 
 template <int RM, int ACT, int CT>
 void launch_few(const Fp8Gemm& p, hipStream_t s) {
-  hipLaunchKernelGGL((fp8_gemm_few_kernel<RM, ACT, CT>), dim3(cdiv(p.N, 16), cdiv(p.M, 16 * RM)), dim3(512), 0, s, p);
+  const dim3 grid(cdiv(p.N, 16), cdiv(p.M, 16 * RM));
+  if (p.tail) hipLaunchKernelGGL((fp8_gemm_few_kernel<RM, true, ACT, CT>), grid, dim3(512), 0, s, p);
+  else hipLaunchKernelGGL((fp8_gemm_few_kernel<RM, false, ACT, CT>), grid, dim3(512), 0, s, p);
 }
 
 int g_force = -1;  // tests and measurements: run this kernel whatever the sizes (fp8_gemm_force)
@@ -570,6 +625,13 @@ double estimate(int k, const Fp8Gemm& p) {
 }
 
 template <int ACT, int CT>
+void launch_big(const Fp8Gemm& p, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv(p.M, 256) * cdiv(p.N, 256)));
+  if (p.tail) hipLaunchKernelGGL((fp8_gemm_big_kernel<true, ACT, CT>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((fp8_gemm_big_kernel<false, ACT, CT>), grid, dim3(256), 0, s, p);
+}
+
+template <int ACT, int CT>
 void launch(const Fp8Gemm& p, hipStream_t s) {
   auto fits = [&](int k) {
     if (k <= K_FEW32) return cdiv(p.M, 16) <= 65535;              // grid.y
@@ -588,7 +650,7 @@ void launch(const Fp8Gemm& p, hipStream_t s) {
     case K_128x64: launch_tile<128, 64, 4, ACT, CT>(p, s); break;
     case K_128_4: launch_tile<128, 128, 4, ACT, CT>(p, s); break;
     case K_128_2: launch_tile<128, 128, 2, ACT, CT>(p, s); break;
-    default: hipLaunchKernelGGL((fp8_gemm_big_kernel<ACT, CT>), dim3((unsigned)(cdiv(p.M, 256) * cdiv(p.N, 256))), dim3(256), 0, s, p);
+    default: launch_big<ACT, CT>(p, s);
   }
 }
 
@@ -604,10 +666,10 @@ void launch_act(const Fp8Gemm& p, int ctype, hipStream_t s) {
 void fp8_gemm_force(int k) { g_force = k; }
 
 int fp8_gemm_launch(const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, void* C,
-                    const float* bias, int M, int N, int nk, long lda, long ldb, int ldsa, int ldsb, int bshift,
+                    const float* bias, int M, int N, int nk, int tail, long lda, long ldb, int ldsa, int ldsb, int bshift,
                     long ldc, int act, int ctype, hipStream_t s) {
   if (M <= 0 || N <= 0 || nk <= 0) return 0;
-  const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, lda, ldb, ldsa, ldsb, bshift, ldc};
+  const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, tail, lda, ldb, ldsa, ldsb, bshift, ldc};
   if (lda > (1 << 22) && cdiv(M, 16) > 65535) return (int)hipErrorInvalidValue;  // (grid of the few-row kernels)
   if (act == ACT_NONE) launch_act<ACT_NONE>(p, ctype, s);
   else if (act == ACT_RELU) launch_act<ACT_RELU>(p, ctype, s);

@@ -31,7 +31,8 @@ def scale_cols(cols: int) -> int:
 class Fp8Blocks:
     """A matrix ``[rows, cols]`` in e4m3 with one scale byte (exponent + 127) for each block of 128 columns.
 
-    ``q``      float8_e4m3fn ``[rows, cols rounded up to 128]``, zeros behind ``cols``;
+    ``q``      float8_e4m3fn ``[rows, cols rounded up to 128]``; what stands behind ``cols`` counts as zeros (the
+               quantisers write zeros there);
     ``scale``  uint8 ``[ceil(rows / tile), blocks rounded up to 4]``;
     ``tile``   rows that share a scale: 1 (activations) or 128 (weights).
 

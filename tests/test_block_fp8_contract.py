@@ -70,3 +70,57 @@ def test_function_transforms_are_refused():
             torch.func.jvp(f, (x,), (torch.ones_like(x),))
         with pytest.raises(Exception):
             torch.vmap(f)(x.view(4, 1, 64))
+
+
+# ---------------------------------------------------------------------------
+# operands that a user lays out
+# ---------------------------------------------------------------------------
+def user_blocks(rows, k, tile, dev, fill, seed):
+    """Small integers under scales of 2^-1, 1 and 2, every byte behind column k and behind the last block's scale
+    ``fill``; and the values this stands for."""
+    g = torch.Generator().manual_seed(seed)
+    kp, nb = fb.padded_cols(k), -(-k // 128)
+    v = torch.randint(-3, 4, (rows, k), generator=g).float()
+    q = torch.full((rows, kp), fill, dtype=torch.uint8)
+    q[:, :k] = v.to(torch.float8_e4m3fn).view(torch.uint8)
+    s = torch.full((-(-rows // tile), fb.scale_cols(k)), fill, dtype=torch.uint8)
+    s[:, :nb] = torch.randint(126, 129, (s.shape[0], nb), generator=g).to(torch.uint8)
+    scale = 2.0 ** (s[:, :nb].double() - 127).repeat_interleave(tile, 0)[:rows].repeat_interleave(128, 1)[:, :k]
+    return fb.Fp8Blocks(q.view(torch.float8_e4m3fn).to(dev), s.to(dev), (rows, k), tile), v.double() * scale
+
+
+def forced(kernel):
+    class Force:
+        def __enter__(self):
+            from pytorch_imageclassification_distributed_amd.ops import hip
+            hip.C.fp8_gemm_force(kernel)
+
+        def __exit__(self, *exc):
+            from pytorch_imageclassification_distributed_amd.ops import hip
+            hip.C.fp8_gemm_force(-1)
+    return Force()
+
+
+TAILS = [1, 15, 16, 17, 63, 64, 100, 127, 129, 200, 255, 257, 384 + 77, 640 + 3, 768 + 113]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("fill", [0x7F, 0xFF, 0x38])  # NaN, -NaN, 1.0
+@pytest.mark.parametrize("k", TAILS)
+def test_bytes_behind_the_last_column_count_as_zeros(dev, fill, k):
+    for tile in (1, 128):
+        a, av = user_blocks(70, k, 1, dev, fill, k)
+        b, bv = user_blocks(150, k, tile, dev, fill, k + 1)
+        assert torch.equal(a.dequantize().double().cpu(), av) and torch.equal(b.dequantize().double().cpu(), bv)
+        assert torch.equal(Fx.matmul_fp8(a, b, out_dtype=torch.float32).double().cpu(), av @ bv.t())
+
+
+@gpu
+@pytest.mark.parametrize("kernel", range(7))
+@pytest.mark.parametrize("k", TAILS)
+def test_bytes_behind_the_last_column_every_kernel(kernel, k):
+    for m, n in ((5, 40), (150, 300), (300, 270)):
+        a, av = user_blocks(m, k, 1, "cuda", 0x7F, k)
+        b, bv = user_blocks(n, k, 128, "cuda", 0xFF, k + 1)
+        with forced(kernel):
+            assert torch.equal(Fx.matmul_fp8(a, b, out_dtype=torch.float32).double().cpu(), av @ bv.t()), (m, n)
