@@ -611,7 +611,8 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* __restrict_
     const long r = i / N;
     const int c = (int)(i - r * N);
     const float v = __builtin_amdgcn_cvt_f32_fp8((int)q[r * ldq + c], 0);
-    y[i] = from_f<T>(ldexpf(v, (int)sc[(r / tile) * ldsc + (c >> 7)] - 127));
+    const int s = sc[(r / tile) * ldsc + (c >> 7)];
+    y[i] = from_f<T>(s == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(v, s - 127));  // (an E8M0 byte of 255 is a NaN)
   }
 }
 

@@ -33,7 +33,8 @@ class Fp8Blocks:
 
     ``q``      float8_e4m3fn ``[rows, cols rounded up to 128]``; what stands behind ``cols`` counts as zeros (the
                quantisers write zeros there);
-    ``scale``  uint8 ``[ceil(rows / tile), blocks rounded up to 4]``;
+    ``scale``  uint8 ``[ceil(rows / tile), blocks rounded up to 4]``; 255 makes its block NaN; bytes behind the last
+               block are not read for their value;
     ``tile``   rows that share a scale: 1 (activations) or 128 (weights).
 
     Made by ``quantize_fp8`` / ``quantize_fp8_weight`` / ``rms_norm_fp8``, or from a checkpoint's 8-bit weights."""
@@ -116,9 +117,9 @@ def block_exponent(amax: torch.Tensor) -> torch.Tensor:
 
 
 def _pow2(e: torch.Tensor) -> torch.Tensor:
-    """2^e in float32, exactly, for -127 <= e <= 127."""
+    """2^e in float32, exactly, for -127 <= e <= 127; NaN for 128 (the E8M0 byte 255)."""
     normal = ((e.to(torch.int32) + 127).clamp(min=1) << 23).view(torch.float32)
-    return torch.where(e < -126, normal / 2, normal)
+    return torch.where(e < -126, normal / 2, torch.where(e > 127, torch.nan, normal))
 
 
 def _finite_amax(v, dims, keepdim=True):

@@ -124,3 +124,21 @@ def test_bytes_behind_the_last_column_every_kernel(kernel, k):
         b, bv = user_blocks(n, k, 128, "cuda", 0xFF, k + 1)
         with forced(kernel):
             assert torch.equal(Fx.matmul_fp8(a, b, out_dtype=torch.float32).double().cpu(), av @ bv.t()), (m, n)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_scale_byte_of_255_is_a_nan(dev):
+    a, av = user_blocks(40, 256, 1, dev, 0, 5)
+    b, bv = user_blocks(256, 256, 128, dev, 0, 6)
+    a.q[3, 130] = b.q[200, 7] = 1.0  # (a zero times NaN is one as well, but not every adder says so)
+    av, bv = a.dequantize().double().cpu(), b.dequantize().double().cpu()
+    a.scale[3, 1] = 255
+    b.scale[1, 0] = 255
+    assert bool(a.dequantize()[3, 128:].isnan().all()) and bool(a.dequantize()[3, :128].isfinite().all())
+    assert bool(b.dequantize()[128:, :128].isnan().all()) and bool(b.dequantize()[:128].isfinite().all())
+    y = Fx.matmul_fp8(a, b, out_dtype=torch.float32).double().cpu()
+    want = av @ bv.t()
+    bad = torch.zeros_like(want, dtype=torch.bool)
+    bad[3] = True
+    bad[:, 128:] = True
+    assert bool(y[bad].isnan().all()) and torch.equal(y[~bad], want[~bad])
