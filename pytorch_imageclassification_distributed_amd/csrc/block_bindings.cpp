@@ -34,9 +34,11 @@ int quant_tiles_launch(const void*, uint8_t*, uint8_t*, uint8_t*, uint8_t*, int,
                        hipStream_t);
 int dequant_launch(const uint8_t*, const uint8_t*, void*, long, int, long, int, int, int, hipStream_t);
 void rows_grad_force(int);
-int rows_grad_plan(int, int, int, int, int*);
+int rows_grad_forced();
+int rows_grad_plan(int, int, int, int, int, int*);
 int rows_grad_launch(const bf16_t*, const bf16_t*, float*, float*, int, int, int, int, int, int, int, hipStream_t);
 void fp8_gemm_force(int);
+int fp8_gemm_plan(int, int, int, int);
 int fp8_gemm_launch(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, const float*, int, int, int,
                     int, long, long, int, int, int, long, int, int, hipStream_t);
 
@@ -456,14 +458,14 @@ Tensor op_matmul(const Tensor& a, const Tensor& as, const Tensor& b, const Tenso
 }
 
 // dw[n][k] = sum over the m rows of dy[row][n] x[row][k]; dy, x: bf16, widths n, k rounded up to 8
-void rows_grad(const bf16_t* dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k) {
+void rows_grad(const bf16_t* dy, const Tensor& x, const Tensor& dw, int64_t m, int64_t n, int64_t k, int force) {
   const c10::DeviceGuard guard(dw.device());
   const int64_t ldy = (n + 7) / 8 * 8, ldx = (k + 7) / 8 * 8;
   typed(x, dw, at::kBFloat16, m * ldx, "x");
   TORCH_CHECK(dw.scalar_type() == at::kFloat && dw.is_contiguous() && dw.numel() == n * k && ((uintptr_t)dw.data_ptr() & 15) == 0,
               "linear_fp8: weight gradient must be contiguous float32");
   int tile = 0;
-  const int splits = rows_grad_plan((int)m, (int)n, (int)k, (int)std::max(ldy, ldx), &tile);
+  const int splits = rows_grad_plan((int)m, (int)n, (int)k, (int)std::max(ldy, ldx), force, &tile);
   TORCH_CHECK(splits > 0, "linear_fp8: rows too wide for the weight gradient");
   Tensor slabs;
   if (splits > 1) slabs = fresh({splits * n * k}, dw, at::kFloat);
@@ -544,6 +546,7 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
     ctx->saved_data["wtype"] = (int64_t)weight.scalar_type();
     ctx->saved_data["bias"] = has(bias);
     ctx->saved_data["btype"] = has(bias) ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat;
+    ctx->saved_data["tile"] = (int64_t)rows_grad_forced();
     ctx->saved_data["wslot"] = std::move(wslot);
     ctx->saved_data["bslot"] = std::move(bslot);
     return o.y;
@@ -587,7 +590,8 @@ struct LinearFp8Node : torch::autograd::Function<LinearFp8Node> {
     }
     if (nw) {
       dw = slot_or_empty(ctx->saved_data["wslot"], {n, k}, dy);
-      rows_grad(copied ? (const bf16_t*)(p + copy) : (const bf16_t*)dy.data_ptr(), xb, dw, m, n, k);
+      rows_grad(copied ? (const bf16_t*)(p + copy) : (const bf16_t*)dy.data_ptr(), xb, dw, m, n, k,
+                (int)ctx->saved_data["tile"].toInt());
       const auto t = (at::ScalarType)ctx->saved_data["wtype"].toInt();
       if (t != at::kFloat) dw = dw.to(t);
     }
@@ -625,6 +629,13 @@ void register_block_ops(pybind11::module& m) {
     return op_matmul(a, as, b, bs, bias, n, k, btile, act, torch::python::detail::py_object_to_dtype(dtype));
   });
   m.def("linear_fp8", &op_linear_fp8);
+  // which kernel runs: forced for the calling thread (tests), and the choice for given sizes
   m.def("fp8_gemm_force", &fp8_gemm_force);
+  m.def("fp8_gemm_plan", [](int m, int n, int k, int btile) { return fp8_gemm_plan(m, n, (int)blocks_of(k), btile == 128 ? 7 : 0); });
   m.def("rows_grad_force", &rows_grad_force);
+  m.def("rows_grad_plan", [](int m, int n, int k) {
+    int tile = 0;
+    const int splits = rows_grad_plan(m, n, k, std::max((n + 7) / 8, (k + 7) / 8) * 8, rows_grad_forced(), &tile);
+    return std::make_tuple(tile, splits);
+  });
 }

@@ -596,7 +596,7 @@ void launch_few(const Fp8Gemm& p, hipStream_t s) {
   else hipLaunchKernelGGL((fp8_gemm_few_kernel<RM, false, ACT, CT>), grid, dim3(512), 0, s, p);
 }
 
-int g_force = -1;  // tests and measurements: run this kernel whatever the sizes (fp8_gemm_force)
+thread_local int g_force = -1;  // tests and measurements: this thread's calls run this kernel where it fits (fp8_gemm_force)
 
 // Which kernel: the one whose time this estimates lowest, in us, from what each measured on 256 CUs - a round of blocks
 // costs so much a k-step, plus its first loads and its outputs.  Measured (K 4096 unless given; kernel: us):
@@ -631,49 +631,62 @@ void launch_big(const Fp8Gemm& p, hipStream_t s) {
   else hipLaunchKernelGGL((fp8_gemm_big_kernel<false, ACT, CT>), grid, dim3(256), 0, s, p);
 }
 
-template <int ACT, int CT>
-void launch(const Fp8Gemm& p, hipStream_t s) {
+// the kernel of a launch; -1: none takes these sizes
+int pick_kernel(const Fp8Gemm& p) {
   auto fits = [&](int k) {
     if (k <= K_FEW32) return cdiv(p.M, 16) <= 65535;              // grid.y
     if (p.lda > (1 << 22) || p.ldb > (1 << 22)) return false;     // 32-bit offsets inside a tile of 256 rows
     return k != K_256 || p.bshift == 7;                           // it takes one scale for its 128 columns
   };
-  int pick = K_FEW32;
+  if (g_force >= 0 && g_force < K_COUNT && fits(g_force)) return g_force;
+  int pick = -1;
   double best = 1e30;
   for (int k = 0; k < K_COUNT; ++k)
     if (fits(k) && estimate(k, p) < best) best = estimate(pick = k, p);
-  if (g_force >= 0 && g_force < K_COUNT && fits(g_force)) pick = g_force;
-  switch (pick) {
+  return pick;
+}
+
+template <int ACT, int CT>
+int launch(const Fp8Gemm& p, hipStream_t s) {
+  switch (pick_kernel(p)) {
     case K_FEW16: launch_few<1, ACT, CT>(p, s); break;
     case K_FEW32: launch_few<2, ACT, CT>(p, s); break;
     case K_64: launch_tile<64, 64, 4, ACT, CT>(p, s); break;
     case K_128x64: launch_tile<128, 64, 4, ACT, CT>(p, s); break;
     case K_128_4: launch_tile<128, 128, 4, ACT, CT>(p, s); break;
     case K_128_2: launch_tile<128, 128, 2, ACT, CT>(p, s); break;
-    default: launch_big<ACT, CT>(p, s);
+    case K_256: launch_big<ACT, CT>(p, s); break;
+    default: return (int)hipErrorInvalidValue;
   }
+  HIP_CHECK_LAUNCH();
+  return 0;
 }
 
 template <int ACT>
-void launch_act(const Fp8Gemm& p, int ctype, hipStream_t s) {
-  if (ctype == C_BF16) launch<ACT, C_BF16>(p, s);
-  else if (ctype == C_F16) launch<ACT, C_F16>(p, s);
-  else launch<ACT, C_F32>(p, s);
+int launch_act(const Fp8Gemm& p, int ctype, hipStream_t s) {
+  if (ctype == C_BF16) return launch<ACT, C_BF16>(p, s);
+  if (ctype == C_F16) return launch<ACT, C_F16>(p, s);
+  return launch<ACT, C_F32>(p, s);
 }
 
 }  // namespace
 
 void fp8_gemm_force(int k) { g_force = k; }
 
+// the kernel that a call of these sizes would run in this thread
+int fp8_gemm_plan(int M, int N, int nk, int bshift) {
+  Fp8Gemm p{};
+  p.M = M; p.N = N; p.nk = nk; p.bshift = bshift;
+  p.lda = p.ldb = (long)nk * 128;
+  return pick_kernel(p);
+}
+
 int fp8_gemm_launch(const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, void* C,
                     const float* bias, int M, int N, int nk, int tail, long lda, long ldb, int ldsa, int ldsb, int bshift,
                     long ldc, int act, int ctype, hipStream_t s) {
   if (M <= 0 || N <= 0 || nk <= 0) return 0;
   const Fp8Gemm p{A, As, B, Bs, C, bias, M, N, nk, tail, lda, ldb, ldsa, ldsb, bshift, ldc};
-  if (lda > (1 << 22) && cdiv(M, 16) > 65535) return (int)hipErrorInvalidValue;  // (grid of the few-row kernels)
-  if (act == ACT_NONE) launch_act<ACT_NONE>(p, ctype, s);
-  else if (act == ACT_RELU) launch_act<ACT_RELU>(p, ctype, s);
-  else launch_act<ACT_SILU>(p, ctype, s);
-  HIP_CHECK_LAUNCH();
-  return 0;
+  if (act == ACT_NONE) return launch_act<ACT_NONE>(p, ctype, s);
+  if (act == ACT_RELU) return launch_act<ACT_RELU>(p, ctype, s);
+  return launch_act<ACT_SILU>(p, ctype, s);
 }

@@ -333,15 +333,18 @@ int stages_of(int M) { return (M + STAGE_ROWS - 1) / STAGE_ROWS; }
 
 }  // namespace
 
-static int g_force = 0;  // tests: this tile whatever the sizes (rows_grad_force)
+// tests: the tile of the weight gradients of this thread's forward calls, whatever the sizes (0: by estimate).  The
+// backward pass runs in a thread of its own: a call's node takes the value along.
+static thread_local int g_force = 0;
 void rows_grad_force(int tile) { g_force = tile; }
+int rows_grad_forced() { return g_force; }
 
 // The tile's width and the row splits: few tiles over few rows leave CUs idle, slabs cost their bytes twice.  Estimated
 // time in us: a round of 256 blocks takes 1.45 a stage and 14 for first loads and outputs, with the small tile 0.5 and 7
 // (4096 x 4096 x 4096: 105 and 162 us; 300 x 4096 x 4096: 22 and 31; 4096 x 2048 x 2048: 50 and 38); the slabs' sum
 // 4 TB/s.  At least as many splits as keep the byte offsets inside one (and the three stages past its end) in 32 bits; 0
 // where even the shortest split is too long.
-int rows_grad_plan(int M, int N, int K, int ld, int* tile) {
+int rows_grad_plan(int M, int N, int K, int ld, int force, int* tile) {
   const int stages = stages_of(M);
   *tile = 256;
   if (stages == 0) return 1;
@@ -351,7 +354,7 @@ int rows_grad_plan(int M, int N, int K, int ld, int* tile) {
   int best = fewest;
   double least = 1e30;
   for (int t = 128; t <= 256; t += 128) {
-    if (g_force && g_force != t) continue;
+    if (force && force != t) continue;
     const long tiles = (long)cdiv(N, t) * cdiv(K, t);
     for (int s = fewest; s <= (fewest > 64 ? fewest : 64) && s <= stages; ++s) {
       const double rounds = (double)((tiles * s + 255) / 256), per = (stages + s - 1) / s;

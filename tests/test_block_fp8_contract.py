@@ -142,3 +142,105 @@ def test_a_scale_byte_of_255_is_a_nan(dev):
     bad[3] = True
     bad[:, 128:] = True
     assert bool(y[bad].isnan().all()) and torch.equal(y[~bad], want[~bad])
+
+
+# ---------------------------------------------------------------------------
+# the choice of a kernel
+# ---------------------------------------------------------------------------
+def in_another_thread(f):
+    import threading
+    got = []
+    t = threading.Thread(target=lambda: got.append(f()))
+    t.start()
+    t.join()
+    return got[0]
+
+
+def test_forcing_a_kernel_is_the_threads_own():
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    C = hip.C
+    free = C.fp8_gemm_plan(8192, 8192, 4096, 128), C.rows_grad_plan(8192, 8192, 4096)
+    assert free[0] == 6 and free[1][0] == 256
+    try:
+        C.fp8_gemm_force(0)
+        C.rows_grad_force(128)
+        assert C.fp8_gemm_plan(8192, 8192, 4096, 128) == 0 and C.rows_grad_plan(8192, 8192, 4096)[0] == 128
+        assert in_another_thread(lambda: (C.fp8_gemm_plan(8192, 8192, 4096, 128), C.rows_grad_plan(8192, 8192, 4096))) == free
+    finally:
+        C.fp8_gemm_force(-1)
+        C.rows_grad_force(0)
+    assert (C.fp8_gemm_plan(8192, 8192, 4096, 128), C.rows_grad_plan(8192, 8192, 4096)) == free
+
+
+@pytest.mark.parametrize("kernel", range(7))
+def test_a_forced_kernel_is_the_one_that_runs(kernel):
+    """The sizes of the other tests of every kernel; the large tile takes weights with 128 x 128 scales only."""
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    with forced(kernel):
+        for m, n, k in ((1, 16, 128), (5, 100, 130), (70, 130, 1000), (150, 260, 1281), (300, 515, 640), (257, 129, 2176)):
+            assert hip.C.fp8_gemm_plan(m, n, k, 128) == kernel
+            assert (hip.C.fp8_gemm_plan(m, n, k, 1) == kernel) == (kernel != 6)
+
+
+@gpu
+def test_a_forced_weight_gradient_tile_reaches_the_backward_thread():
+    """Each tile splits the rows its own way: at a size where float32 sums differ, a forced tile gives its own bits."""
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    lin = nn.Linear(300, 200).cuda()
+    x, dy = rand((9000, 300), torch.bfloat16, "cuda", 11), rand((9000, 200), torch.bfloat16, "cuda", 12)
+    got = {}
+    for tile in (128, 256, 128, 256):
+        hip.C.rows_grad_force(tile)
+        try:
+            plan = hip.C.rows_grad_plan(9000, 200, 300)
+            y = Fx.linear_fp8(x, lin)
+        finally:
+            hip.C.rows_grad_force(0)
+        (dw,) = torch.autograd.grad(y, (lin.weight,), dy)
+        assert plan[0] == tile and torch.equal(got.setdefault(plan, dw), dw)
+    a, b = got.values()
+    assert len(got) == 2 and not torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 16, 17, 33, 64, 129, 256, 299])
+def test_rows_do_not_depend_on_the_rows_around_them(m):
+    """The first m rows alone against the same rows of a call with 300: the kernels differ, and with them the order of the
+    float32 sums and where the matrix instruction cuts - each within 2^-12 of the sum of magnitudes."""
+    x, w = rand((300, 1152), torch.bfloat16, "cuda", 74), rand((272, 1152), torch.float32, "cuda", 75, 0.03)
+    a, b = Fx.quantize_fp8(x), Fx.quantize_fp8_weight(w)
+    part = Fx.matmul_fp8(Fx.quantize_fp8(x[:m]), b, out_dtype=torch.float32)
+    whole = Fx.matmul_fp8(a, b, out_dtype=torch.float32)[:m]
+    mag = a.dequantize()[:m].double().abs() @ b.dequantize().double().abs().t()
+    assert bool(((part - whole).double().abs() <= 2 * 2.0**-12 * mag).all())
+
+
+@gpu
+def test_gpu_tensors_run_the_kernels(monkeypatch):
+    """Every operator hands GPU tensors to its kernels' entry point, once a call."""
+    from pytorch_imageclassification_distributed_amd.ops._hip import block
+    calls = []
+
+    class Counting:
+        def __init__(self, C):
+            self.C = C
+
+        def __getattr__(self, name):
+            calls.append(name)
+            return getattr(self.C, name)
+    monkeypatch.setattr(block, "C", Counting(block.C))
+    x = rand((4, 64), torch.float32, "cuda", 3)
+    norm, lin = nn.RMSNorm(64).cuda(), nn.Linear(64, 8).cuda()
+    with torch.no_grad():
+        for name, f in (("dropout_counter", lambda: Fx.dropout_counter(x, 0.5, seed=1)), ("rms_norm", lambda: Fx.rms_norm(x, norm)),
+                        ("rms_norm_fp8", lambda: Fx.rms_norm_fp8(x, norm)), ("quantize_fp8_rows", lambda: Fx.quantize_fp8(x)),
+                        ("quantize_fp8_tiles", lambda: Fx.quantize_fp8_weight(lin.weight)),
+                        ("linear_fp8", lambda: Fx.linear_fp8(x, lin))):
+            f()
+            assert calls == [name]
+            calls.clear()
+        q, w = Fx.quantize_fp8(x), Fx.quantize_fp8_weight(lin.weight)
+        calls.clear()
+        Fx.matmul_fp8(q, w)
+        q.dequantize()
+        assert calls == ["matmul_fp8", "dequantize_fp8"]
