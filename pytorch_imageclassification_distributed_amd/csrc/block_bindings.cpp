@@ -217,8 +217,8 @@ void fp8_gemm(Tensor a, Tensor as, Tensor b, Tensor bs, Tensor c, OT bias, int64
   blocks(a, as, a, M, K, 1);
   blocks(b, bs, a, N, K, btile);
   typed(bias, a, at::kFloat, N, "bias");
-  // one block a 128 x 128 tile or smaller
-  TORCH_CHECK(((M + 15) / 16) * ((N + 15) / 16) < (1LL << 31), "matmul_fp8: grid too large");
+  TORCH_CHECK(M * N == 0 || fp8_gemm_plan((int)M, (int)N, (int)(a.size(1) / 128), btile == 128 ? 7 : 0) >= 0,
+              "matmul_fp8: no kernel takes [", M, ", ", K, "] x [", N, ", ", K, "]: too large");
   ok(fp8_gemm_launch((const uint8_t*)a.data_ptr(), as.data_ptr<uint8_t>(), (const uint8_t*)b.data_ptr(),
                      bs.data_ptr<uint8_t>(), c.data_ptr(), (const float*)raw(bias), (int)M, (int)N, (int)(a.size(1) / 128),
                      (int)(K % 128), a.size(1), b.size(1), (int)as.size(1), (int)bs.size(1), btile == 128 ? 7 : 0, N, act, code,

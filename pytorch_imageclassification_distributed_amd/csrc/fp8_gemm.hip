@@ -633,8 +633,12 @@ void launch_big(const Fp8Gemm& p, hipStream_t s) {
 
 // the kernel of a launch; -1: none takes these sizes
 int pick_kernel(const Fp8Gemm& p) {
+  // (a grid holds fewer than 2^32 threads a dimension, and 65535 blocks in its second)
+  auto tiles = [&](long m, long n) { return ((p.M + m - 1) / m) * ((p.N + n - 1) / n); };
   auto fits = [&](int k) {
-    if (k <= K_FEW32) return cdiv(p.M, 16) <= 65535;              // grid.y
+    if (k <= K_FEW32) return tiles(1L << 40, 16) < (1L << 23) && (p.M + 15L) / 16 <= 65535;  // 512 threads a block
+    const int bm = k == K_64 ? 64 : k == K_256 ? 256 : 128, bn = k <= K_128x64 ? 64 : k == K_256 ? 256 : 128;
+    if (tiles(bm, bn) >= (1L << 24)) return false;                // 256
     if (p.lda > (1 << 22) || p.ldb > (1 << 22)) return false;     // 32-bit offsets inside a tile of 256 rows
     return k != K_256 || p.bshift == 7;                           // it takes one scale for its 128 columns
   };

@@ -244,3 +244,38 @@ def test_gpu_tensors_run_the_kernels(monkeypatch):
         Fx.matmul_fp8(q, w)
         q.dequantize()
         assert calls == ["matmul_fp8", "dequantize_fp8"]
+
+
+def test_the_choice_keeps_within_a_grids_limits():
+    """At most 2^32 - 1 threads along a grid's first dimension, 65535 blocks along its second; 32-bit offsets in a tile."""
+    from pytorch_imageclassification_distributed_amd.ops import hip
+    plan = hip.C.fp8_gemm_plan
+    sizes = {0: (16, 16, 512), 1: (32, 16, 512), 2: (64, 64, 256), 3: (128, 64, 256), 4: (128, 128, 256), 5: (128, 128, 256),
+             6: (256, 256, 256)}
+    for m, n, k in ((1, 2**27 - 16, 128), (1, 2**27, 128), (1, 2**29, 128), (16, 2**28, 128), (2**20 + 16, 16, 2**23), (2**29, 16, 128),
+                    (2**18, 2**18, 128), (2**21, 2**14, 128), (64, 2**26, 256), (2**17, 2**17, 4096)):
+        for tile in (1, 128):
+            pick = plan(m, n, k, tile)
+            if pick < 0:
+                assert k > 2**22 or m * n >= 2**36
+                continue
+            bm, bn, threads = sizes[pick]
+            gx, gy = -(-n // bn), -(-m // bm)
+            if pick <= 1:
+                assert gx * threads < 2**32 and gy <= 65535, (m, n, k, pick)
+            else:
+                assert gx * gy * threads < 2**32 and k <= 2**22, (m, n, k, pick)
+    assert plan(1, 2**29, 128, 128) > 1 and plan(2**20 + 16, 16, 2**23, 128) == -1
+
+
+@gpu
+def test_more_weight_rows_than_the_few_row_kernels_grid():
+    """2^27 + 5 outputs of one row (17 GB of weights): blocks of 512 threads, one for 16 outputs, would pass 2^32 threads."""
+    n = 2**27 + 5
+    q = torch.zeros(n, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    rows = torch.tensor([0, 15, 16, 2**26 + 3, 2**27 - 1, 2**27, n - 1], device="cuda")
+    q.view(torch.uint8)[rows] = (torch.arange(1, 8, device="cuda").float()).to(torch.float8_e4m3fn).view(torch.uint8)[:, None]
+    w = fb.Fp8Blocks(q, torch.full((-(-n // 128), 4), 127, dtype=torch.uint8, device="cuda"), (n, 128), 128)
+    y = Fx.matmul_fp8(Fx.quantize_fp8(torch.ones(1, 128, device="cuda")), w, out_dtype=torch.float32)[0]
+    assert torch.equal(y[rows].cpu(), 128 * torch.arange(1, 8).float())
+    assert int((y != 0).sum()) == 7
