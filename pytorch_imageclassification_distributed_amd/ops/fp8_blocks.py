@@ -226,7 +226,7 @@ class _RmsNorm(torch.autograd.Function):
         f, a = h.float(), dy.float()
         dw = None
         if weight is not None:
-            dw = (a * f * inv).flatten(0, -2).sum(0).to(weight.dtype)
+            dw = (a * f * inv).reshape(-1, f.shape[-1]).sum(0).to(weight.dtype)
             a = a * weight.float()
         g = inv * (a - f * inv.square() * (a * f).mean(-1, keepdim=True))
         if dh is not None:

@@ -279,3 +279,22 @@ def test_more_weight_rows_than_the_few_row_kernels_grid():
     y = Fx.matmul_fp8(Fx.quantize_fp8(torch.ones(1, 128, device="cuda")), w, out_dtype=torch.float32)[0]
     assert torch.equal(y[rows].cpu(), 128 * torch.arange(1, 8).float())
     assert int((y != 0).sum()) == 7
+
+
+# ---------------------------------------------------------------------------
+# shapes, seeds, parameters
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", DEVICES)
+def test_one_dimensional_rows(dev):
+    """x of one dimension is one row, in both directions."""
+    x, r, dy, dh = (rand((40,), torch.bfloat16, dev, s) for s in range(20, 24))
+    norm, lin = nn.RMSNorm(40).to(dev), nn.Linear(40, 6).to(dev)
+
+    def step(shape):
+        xx, rr = (v.view(shape).clone().requires_grad_(True) for v in (x, r))
+        y, h = Fx.rms_norm(xx, norm, residual=rr, p=0.25, seed=2)
+        z = Fx.linear_fp8(y, lin, "relu")
+        return [y, h, z] + list(torch.autograd.grad((y, h, z.sum()), (xx, rr, norm.weight, lin.weight, lin.bias),
+                                                    (dy.view(shape), dh.view(shape), torch.ones((), dtype=z.dtype, device=dev))))
+    for a, b in zip(step((40,)), step((1, 40))):
+        assert torch.equal(a.reshape(b.shape), b)
