@@ -497,6 +497,9 @@ LinearOut linear_forward(const Tensor& x, const Tensor& weight, const OT& bias, 
   const int64_t m = x.size(0), k = x.size(1), n = weight.size(0);
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) == k && weight.device() == x.device(), "linear_fp8: weight shape");
   TORCH_CHECK(m < (1LL << 30) && n >= 1 && n < (1LL << 23) - 128 && k >= 1 && k < (1LL << 23) - 128, "linear_fp8: size");
+  int tile = 0;  // (a width whose weight gradient no launch takes is refused here, not after the forward pass)
+  TORCH_CHECK(!need_w || rows_grad_plan((int)m, (int)n, (int)k, (int)((std::max(n, k) + 7) / 8 * 8), rows_grad_forced(), &tile) > 0,
+              "linear_fp8: rows too wide for the weight gradient");
   const int tx = type_code(x, "x"), tw = type_code(weight, "weight");
   const OT b = f32(bias);
   typed(b, x, at::kFloat, n, "bias");

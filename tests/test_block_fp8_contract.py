@@ -298,3 +298,15 @@ def test_one_dimensional_rows(dev):
                                                     (dy.view(shape), dh.view(shape), torch.ones((), dtype=z.dtype, device=dev))))
     for a, b in zip(step((40,)), step((1, 40))):
         assert torch.equal(a.reshape(b.shape), b)
+
+
+@gpu
+def test_too_wide_for_the_weight_gradient_is_refused_before_the_forward_pass():
+    k = 3_400_000  # (64 + 4 x 64 rows of it pass 32-bit byte offsets)
+    lin = nn.Linear(k, 1, device="cuda", dtype=torch.bfloat16)
+    x = torch.ones(2, k, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="too wide"):
+        Fx.linear_fp8(x, lin)
+    lin.weight.requires_grad_(False)  # the other gradients do not need it
+    dx, db = torch.autograd.grad(Fx.linear_fp8(x, lin).sum(), (x, lin.bias))
+    assert dx.shape == x.shape and float(db) == 2
