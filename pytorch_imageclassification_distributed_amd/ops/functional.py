@@ -406,8 +406,10 @@ def linear_fp8(x, lin, act=None):
         raise NotImplementedError(act)
     if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"linear_fp8: x {tuple(x.shape)} does not fit weight {tuple(w.shape)}")
-    if w.shape[0] < 1 or w.shape[1] < 1 or w.dtype not in FLOATS or (b is not None and b.dtype not in FLOATS):
+    if w.shape[0] < 1 or w.shape[1] < 1 or w.dtype not in FLOATS:
         raise ValueError(f"linear_fp8: weight {w.dtype} {tuple(w.shape)}")
+    if b is not None and (b.dtype not in FLOATS or tuple(b.shape) != (w.shape[0],)):
+        raise ValueError(f"linear_fp8: bias must be [{w.shape[0]}], got {b.dtype} {tuple(b.shape)}")
     if w.device != x.device or (b is not None and b.device != x.device):
         raise ValueError(f"linear_fp8: x on {x.device}, weight on {w.device}")
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])  # (a reshape or view is an autograd node more, 8 us a call)

@@ -310,3 +310,13 @@ def test_too_wide_for_the_weight_gradient_is_refused_before_the_forward_pass():
     lin.weight.requires_grad_(False)  # the other gradients do not need it
     dx, db = torch.autograd.grad(Fx.linear_fp8(x, lin).sum(), (x, lin.bias))
     assert dx.shape == x.shape and float(db) == 2
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("shape", [(9,), (7,), (1,), (8, 1), ()])
+def test_linear_refuses_a_bias_of_another_size(dev, shape):
+    """Neither read in part (a longer one), nor spread (one value)."""
+    lin = nn.Linear(16, 8).to(dev)
+    lin.bias = nn.Parameter(torch.zeros(shape, device=dev))
+    with pytest.raises(ValueError, match="bias"):
+        Fx.linear_fp8(torch.zeros(3, 16, device=dev), lin)
