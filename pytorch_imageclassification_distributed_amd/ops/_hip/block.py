@@ -7,6 +7,7 @@ so calls may run on any stream, at once, and inside a captured graph.
 from __future__ import annotations
 
 import functools
+import operator
 
 import torch
 
@@ -22,7 +23,7 @@ def _drop_state(dev, seed, offset):
         return torch.randint(0, 2**63 - 1, (2,), device=dev, dtype=torch.int64), 0, 0
     if torch.is_tensor(seed):
         return seed, 0, 0
-    return None, seed, offset
+    return None, operator.index(seed), operator.index(offset)
 
 
 def _slot(p):

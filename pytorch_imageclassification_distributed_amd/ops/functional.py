@@ -19,6 +19,7 @@ GPU path fuse conv -> BN -> (+residual) -> activation.
 from __future__ import annotations
 
 import math
+import operator
 import os
 
 import torch
@@ -251,7 +252,7 @@ def _check_drop(name, x, p, seed, offset):
     elif seed is None:
         if offset != 0:
             raise ValueError(f"{name}: offset without a seed")
-    elif not (0 <= int(seed) < 2**64 and 0 <= int(offset) < 2**64):
+    elif not (0 <= operator.index(seed) < 2**64 and 0 <= operator.index(offset) < 2**64):  # (TypeError: not an integer)
         raise ValueError(f"{name}: seed and offset are 64-bit unsigned, got {seed}, {offset}")
     return drop_threshold(p)
 
@@ -262,7 +263,7 @@ def _seed_values(seed, offset):
         seed = torch.randint(0, 2**63 - 1, (2,), dtype=torch.int64)
     if torch.is_tensor(seed):
         seed, offset = (v % 2**64 for v in seed.tolist())
-    return int(seed), int(offset)
+    return operator.index(seed), operator.index(offset)
 
 
 def dropout_counter(x, p, training=True, seed=None, offset=0, residual=None):

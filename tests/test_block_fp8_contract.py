@@ -320,3 +320,18 @@ def test_linear_refuses_a_bias_of_another_size(dev, shape):
     lin.bias = nn.Parameter(torch.zeros(shape, device=dev))
     with pytest.raises(ValueError, match="bias"):
         Fx.linear_fp8(torch.zeros(3, 16, device=dev), lin)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_seeds_are_integers(dev):
+    """Any integer type; a fraction is refused, not cut."""
+    import numpy as np
+    x = torch.ones(1000, device=dev)
+    want = Fx.dropout_counter(x, 0.5, seed=2**63 + 5, offset=7)
+    assert torch.equal(Fx.dropout_counter(x, 0.5, seed=np.uint64(2**63 + 5), offset=np.int32(7)), want)
+    norm = nn.RMSNorm(1000).to(dev)
+    for kw in (dict(seed=1.5), dict(seed=2.0), dict(seed="1"), dict(seed=1, offset=0.5)):
+        with pytest.raises(TypeError):
+            Fx.dropout_counter(x, 0.5, **kw)
+        with pytest.raises(TypeError):
+            Fx.rms_norm(x, norm, p=0.5, **kw)
