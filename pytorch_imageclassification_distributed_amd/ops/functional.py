@@ -257,10 +257,10 @@ def _check_drop(name, x, p, seed, offset):
     return drop_threshold(p)
 
 
-def _seed_values(seed, offset):
+def _seed_values(seed, offset, device):
     """Host values for the reference path."""
     if seed is None:
-        seed = torch.randint(0, 2**63 - 1, (2,), dtype=torch.int64)
+        seed = torch.randint(0, 2**63 - 1, (2,), dtype=torch.int64, device=device)
     if torch.is_tensor(seed):
         seed, offset = (v % 2**64 for v in seed.tolist())
     return operator.index(seed), operator.index(offset)
@@ -286,7 +286,7 @@ def dropout_counter(x, p, training=True, seed=None, offset=0, residual=None):
         return _hip().dropout_counter(x, residual, 0, 0, 0) if use_hip(x) else x + residual
     if use_hip(x):
         return _hip().dropout_counter(x, residual, t, seed, offset)
-    y = drop_ref(x.contiguous().float(), t, *_seed_values(seed, offset))
+    y = drop_ref(x.contiguous().float(), t, *_seed_values(seed, offset, x.device))
     return (y if residual is None else y + residual.float()).to(x.dtype)
 
 
@@ -321,7 +321,7 @@ def rms_norm(x, norm, residual=None, p=0.0, training=True, seed=None, offset=0):
     t = _check_drop("rms_norm", x, p, seed, offset) if training else 0
     if use_hip(x):
         return _hip().rms_norm(x, w, eps, residual, t, seed, offset)
-    return rms_norm_ref(x.contiguous(), w, eps, residual, t, *(_seed_values(seed, offset) if t else (0, 0)))
+    return rms_norm_ref(x.contiguous(), w, eps, residual, t, *(_seed_values(seed, offset, x.device) if t else (0, 0)))
 
 
 def rms_norm_fp8(x, norm, residual=None):

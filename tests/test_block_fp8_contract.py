@@ -335,3 +335,21 @@ def test_seeds_are_integers(dev):
             Fx.dropout_counter(x, 0.5, **kw)
         with pytest.raises(TypeError):
             Fx.rms_norm(x, norm, p=0.5, **kw)
+
+
+@gpu
+def test_both_backends_draw_a_seed_from_the_devices_generator():
+    x = torch.ones(4096, device="cuda")
+    keep = Fx.get_backend()
+    got = {}
+    try:
+        for backend in ("hip", "torch"):
+            Fx.set_backend(backend)
+            torch.cuda.manual_seed(5)
+            torch.random.default_generator.manual_seed(len(got))
+            got[backend] = Fx.dropout_counter(x, 0.5), Fx.dropout_counter(x, 0.5)
+    finally:
+        Fx.set_backend(keep)
+    for a, b in zip(*got.values()):
+        assert torch.equal(a, b)
+    assert not torch.equal(*got["hip"])
