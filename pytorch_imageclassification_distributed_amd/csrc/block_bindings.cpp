@@ -337,10 +337,10 @@ struct DropoutCounterNode : torch::autograd::Function<DropoutCounterNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const OT state = some(ctx->get_saved_variables()[0]);
+    const DropArgs d = DropArgs::load(ctx);
     Tensor dx;
-    if (ctx->needs_input_grad(0)) dx = drop_forward(g[0].detach(), OT(), state, DropArgs::load(ctx));
-    variable_list out = no_second({dx});
-    return {out[0], ctx->saved_data["res"].toBool() ? g[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (ctx->needs_input_grad(0)) dx = d.t == 0 ? g[0] : no_second({drop_forward(g[0].detach(), OT(), state, d)})[0];
+    return {dx, ctx->saved_data["res"].toBool() ? g[0] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -396,9 +396,9 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
     const Tensor dy = g[0].defined() ? dense16(g[0].detach()) : at::zeros_like(h);
     const OT dh = res && g[1].defined() ? OT(dense16(g[1].detach())) : OT();
     Tensor dx, dres, part, dw;
-    const bool both = nx || !nr;  // without dropout the two gradients are one tensor
-    if (both) dx = at::empty_like(h);
-    if (nr && (d.t > 0 || !both)) dres = at::empty_like(h);
+    const bool one = d.t == 0;  // without dropout the two gradients are one tensor
+    if (nx || (nr && one)) dx = at::empty_like(h);
+    if (nr && !one) dres = at::empty_like(h);
     if (nw) part = fresh({rms_bwd_blocks(rows, (int)n), n}, h, at::kFloat);
     rms_bwd(dy, h, dh, w, rstd, some(dx), some(dres), some(part), rows, n, state, d.seed, d.offset, (int)d.t);
     if (nw) {
@@ -407,7 +407,7 @@ struct RmsNormNode : torch::autograd::Function<RmsNormNode> {
       const auto wt = (at::ScalarType)ctx->saved_data["wtype"].toInt();
       if (wt != at::kFloat) dw = dw.to(wt);
     }
-    variable_list out = no_second({nx ? dx : Tensor(), nr ? (dres.defined() ? dres : dx) : Tensor(), dw});
+    variable_list out = no_second({nx ? dx : Tensor(), nr ? (one ? dx : dres) : Tensor(), dw});
     return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };

@@ -353,3 +353,46 @@ def test_both_backends_draw_a_seed_from_the_devices_generator():
     for a, b in zip(*got.values()):
         assert torch.equal(a, b)
     assert not torch.equal(*got["hip"])
+
+
+@gpu
+def test_backward_makes_no_gradient_that_nobody_asked_for():
+    """Allocations of a backward pass that only the norm's weight, only the residual, or (in evaluation) a plain sum needs."""
+    n, rows = 1024, 4096
+    big = n * rows * 2  # bytes of a gradient of x
+    norm = nn.RMSNorm(n).cuda()
+    x, r, g = (rand((rows, n), torch.bfloat16, "cuda", s) for s in (31, 32, 33))
+
+    def backward(out, ins):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        base = torch.cuda.memory_allocated()
+        grads = torch.autograd.grad(out, ins, g)
+        return torch.cuda.max_memory_allocated() - base, grads
+    part = 512 * n * 4 + 2**20  # the weight's partial sums
+    full = torch.autograd.grad(Fx.rms_norm(x.requires_grad_(), norm, residual=r.requires_grad_(), p=0.5, seed=1)[0],
+                               (x, r, norm.weight), g)
+    x.requires_grad_(False), r.requires_grad_(False)
+    used, (dw,) = backward(Fx.rms_norm(x, norm, residual=r, p=0.5, seed=1)[0], (norm.weight,))
+    assert used <= part and torch.equal(dw, full[2])
+    norm.requires_grad_(False)
+    rr = r.clone().requires_grad_()
+    used, (dr,) = backward(Fx.rms_norm(x, norm, residual=rr, p=0.5, seed=1)[0], (rr,))
+    assert used <= big + 2**20 and torch.equal(dr, full[1])
+    xx = x.clone().requires_grad_()
+    used, grads = backward(Fx.dropout_counter(xx, 0.5, training=False, residual=rr), (xx, rr))
+    assert used <= 2**20 and all(torch.equal(v, g) for v in grads)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_gradients_of_a_plain_sum_accumulate_apart(dev):
+    """Both leaves of an evaluation sum get the same gradient; what is added to one later does not show in the other."""
+    x, r = (rand((8, 16), torch.float32, dev, s).requires_grad_() for s in (34, 35))
+    g = rand((8, 16), torch.float32, dev, 36)
+    y = Fx.dropout_counter(x, 0.5, training=False, residual=r)
+    y.backward(g)
+    x.grad.add_(1)
+    assert torch.equal(r.grad, g) and torch.equal(x.grad, g + 1)
+    (d,) = torch.autograd.grad(Fx.dropout_counter(x, 0.5, training=False, residual=r).square().sum(), x, create_graph=True)
+    (dd,) = torch.autograd.grad(d.sum(), x)  # (the sum itself can be differentiated again)
+    assert torch.equal(dd, torch.full_like(x, 2))
