@@ -86,6 +86,9 @@ const long long* state_of(const OT& st, const Tensor& x) {
 
 void threshold(int t) { TORCH_CHECK(t >= 0 && t <= 65536, "drop threshold out of range"); }
 
+// a copy where t does not begin at a multiple of `bytes` (a user's blocks may be slices of a checkpoint's buffer)
+Tensor aligned(const Tensor& t, uintptr_t bytes) { return ((uintptr_t)t.data_ptr() & (bytes - 1)) == 0 ? t : t.clone(); }
+
 // [rows, cols] e4m3 with cols a multiple of 128, and its scales
 void blocks(const Tensor& q, const Tensor& sc, const Tensor& x, int64_t rows, int64_t cols, int64_t tile) {
   dense(q, x, "q");
@@ -197,6 +200,8 @@ void quant_tiles(Tensor w, Tensor q, Tensor sc) {
 
 void fp8_dequant(Tensor q, Tensor sc, Tensor y, int64_t tile) {
   const c10::DeviceGuard guard(q.device());
+  q = aligned(q, 16);
+  sc = aligned(sc, 4);
   const int code = type_code(y, "y");
   dense(y, q, "y");
   TORCH_CHECK(y.dim() == 2 && (tile == 1 || tile == 128) && y.size(1) < (1LL << 31), "dequantize: shape");
@@ -453,7 +458,7 @@ std::tuple<Tensor, Tensor> op_quantize_tiles(const Tensor& w_) {
 Tensor op_matmul(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, const OT& bias, int64_t n, int64_t k,
                  int64_t btile, int64_t act, at::ScalarType out) {
   Tensor c = fresh({a.size(0), n}, a, out);
-  fp8_gemm(a, as, b, bs, c, f32(bias), k, btile, (int)act);
+  fp8_gemm(aligned(a, 16), aligned(as, 4), aligned(b, 16), aligned(bs, 4), c, f32(bias), k, btile, (int)act);
   return c;
 }
 

@@ -396,3 +396,87 @@ def test_gradients_of_a_plain_sum_accumulate_apart(dev):
     (d,) = torch.autograd.grad(Fx.dropout_counter(x, 0.5, training=False, residual=r).square().sum(), x, create_graph=True)
     (dd,) = torch.autograd.grad(d.sum(), x)  # (the sum itself can be differentiated again)
     assert torch.equal(dd, torch.full_like(x, 2))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("shift", [1, 2, 8])
+def test_blocks_that_begin_at_any_byte(dev, shift):
+    """Values and scales that are slices of one buffer, as a checkpoint may hold them."""
+    a, av = user_blocks(20, 200, 1, dev, 0, 41)
+    b, bv = user_blocks(150, 200, 128, dev, 0, 42)
+
+    def moved(t):
+        buf = torch.zeros(t.numel() + 16, dtype=torch.uint8, device=dev)
+        v = buf[shift:shift + t.numel()]
+        v.copy_(t.view(torch.uint8).flatten())
+        return v.view(t.dtype).view(t.shape)
+    a2, b2 = (fb.Fp8Blocks(moved(v.q), moved(v.scale), v.shape, v.tile) for v in (a, b))
+    assert a2.q.data_ptr() % 16 == (shift if dev == "cuda" else a2.q.data_ptr() % 16)
+    assert torch.equal(a2.dequantize().double().cpu(), av) and torch.equal(b2.dequantize(), b.dequantize())
+    assert torch.equal(Fx.matmul_fp8(a2, b2, out_dtype=torch.float32).double().cpu(), av @ bv.t())
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+@gpu
+def test_a_layer_used_twice_with_and_without_an_arena():
+    """One norm and one linear layer at two places of a network: their gradients add, also where the first goes into an
+    arena's slot."""
+    from pytorch_imageclassification_distributed_amd.ops.grad_arena import GradArena
+    torch.manual_seed(0)
+    norm, lin = nn.RMSNorm(136).cuda(), nn.Linear(136, 136).cuda()
+    params = [norm.weight, lin.weight, lin.bias]
+    x = rand((70, 136), torch.bfloat16, "cuda", 51)
+
+    def step():
+        for p in params:
+            p.grad = None
+        y, h = Fx.rms_norm(x, norm, residual=x)
+        y, h = Fx.rms_norm(Fx.linear_fp8(y, lin, "relu"), norm, residual=h)
+        (Fx.linear_fp8(y, lin) + h).float().square().sum().backward()
+        return [p.grad.clone() for p in params]
+    plain = step()
+    arena = GradArena(params)
+    try:
+        for _ in range(2):
+            for p in params:
+                p.grad = None
+            arena.begin()
+            for a, b in zip(step(), plain):
+                assert torch.equal(a, b)
+    finally:
+        arena.detach_params()
+
+
+@gpu
+def test_seeds_drawn_in_a_captured_graph():
+    """Every replay draws its own mask from the generator, the same in forward and backward."""
+    x = torch.ones(64, 1000, device="cuda").requires_grad_()
+    norm = nn.RMSNorm(1000).cuda()
+
+    def step():
+        y = Fx.dropout_counter(x, 0.5)
+        z, h = Fx.rms_norm(x, norm, residual=torch.zeros_like(x), p=0.25)
+        return [y.detach(), h.detach()] + list(torch.autograd.grad((y, h), (x,), (torch.ones_like(y), torch.zeros_like(h))))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    seen = []
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        y, h, dx = (v.clone() for v in out)
+        assert set(y.unique().tolist()) == {0.0, 2.0} and torch.equal(dx, y)  # dx of ones through the same mask
+        assert len(h.unique()) == 2
+        assert not any(torch.equal(y, a) or torch.equal(h, b) for a, b in seen)
+        seen.append((y, h))
+        assert set(Fx.dropout_counter(x.detach(), 0.5).unique().tolist()) == {0.0, 2.0}  # (eager work between)
+        torch.cuda.synchronize()
