@@ -481,7 +481,8 @@ void rows_grad(const bf16_t* dy, const Tensor& x, const Tensor& dw, int64_t m, i
 
 // y = act(q(x) q(w)^T + b).  Backward: dx = q(dy) q(w) in 8 bits (the weights' transpose was written beside them; 128 x
 // 128 tiles keep their scale), db in float32, and dw = dy^T x on bf16 operands: weight gradients are summed into float32
-// masters over many steps, and the 8-bit matrix instructions cut their sums at 2^-16 where the bf16 ones keep float32.
+// masters over many steps, and the 8-bit matrix instructions cut their products (fp8_gemm.hip) where the bf16 ones keep
+// float32.
 // The quantised operands of a call live in one buffer (an allocation costs a small call as much as a launch does).
 struct Layout {
   int64_t size = 0;

@@ -480,3 +480,69 @@ def test_seeds_drawn_in_a_captured_graph():
         seen.append((y, h))
         assert set(Fx.dropout_counter(x.detach(), 0.5).unique().tolist()) == {0.0, 2.0}  # (eager work between)
         torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------
+# accuracy
+# ---------------------------------------------------------------------------
+def plain_blocks(v, dev):
+    """e4m3 values as they are (scales of 1)."""
+    q = torch.zeros(v.shape[0], fb.padded_cols(v.shape[1]), dtype=torch.float8_e4m3fn)
+    q[:, :v.shape[1]] = v.to(torch.float8_e4m3fn)
+    return fb.Fp8Blocks(q.to(dev), torch.full((v.shape[0], fb.scale_cols(v.shape[1])), 127, dtype=torch.uint8, device=dev), tuple(v.shape))
+
+
+def cut_bound(a, b):
+    """[M, N]: 7 products of every 8 neighbours lose less than 2^-13 of the group's largest power of two; the groups' sums
+    and the accumulator, cut at float32's last bit: (K / 8 + 8) 2^-23 of the sum of magnitudes."""
+    def power(v):
+        return torch.floor(torch.log2(v.double().abs().clamp(min=2.0**-6)))
+    mag = a.double().abs() @ b.double().abs().t()
+    p = torch.where((a[:, None] * b[None]) == 0, -200.0, power(a)[:, None] + power(b)[None])
+    groups = p.view(a.shape[0], b.shape[0], -1, 8).amax(3)
+    return (7 * 2.0 ** (groups - 13)).sum(2) + (a.shape[1] / 8 + 8) * 2.0**-23 * mag, mag
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kernel", [0, 2, 5, 6])
+def test_what_the_matrix_instruction_cuts(dev, kernel):
+    """Random bytes, and one large product beside seven (or 127) equal ones of every other size: within the bound that the
+    instruction's own cut gives, on normal values within 2^-10 of the sum of magnitudes; the reference path is float32's."""
+    g = torch.Generator().manual_seed(7)
+    vals = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
+    cases = []
+    for k in (128, 384):
+        u = torch.randint(0, 256, (64, k), generator=g)
+        cases.append([torch.where((v & 127) == 127, v - 1, v).to(torch.uint8).view(torch.float8_e4m3fn).float()
+                      for v in (u, u.flip(0).roll(5, 1))])
+    for n in (7, 127):
+        for big in (448.0, 256.0, 1.0, 2.0**-6, 2.0**-9):
+            a = torch.zeros(126, 128)
+            a[:, 0] = big
+            a[:, 1:1 + n] = vals[:, None]
+            cases.append([a, a.clone()])
+            b = a.clone()
+            b[:, 0] = 448.0  # (a subnormal beside the largest value)
+            cases.append([a, b])
+    worst = 0.0
+    if dev == "cpu" and kernel:
+        pytest.skip("one reference path")
+    for a, b in cases:
+        qa = plain_blocks(a, dev)
+        qb = plain_blocks(b, dev)
+        if kernel == 6:  # (the large tile takes 128 x 128 scales: the same, all 1)
+            qb = fb.Fp8Blocks(qb.q, qb.scale[:1].contiguous(), qb.shape, 128)
+        import contextlib
+        with (forced(kernel) if dev == "cuda" else contextlib.nullcontext()):
+            y = Fx.matmul_fp8(qa, qb, out_dtype=torch.float32).double().cpu()
+        err = (y - a.double() @ b.double().t()).abs()
+        bound, mag = cut_bound(a, b)
+        if dev == "cpu":
+            assert bool((err <= (a.shape[1] + 2) * 2.0**-24 * mag).all())
+            continue
+        assert bool((err <= bound).all()), float((err / bound).max())
+        normal = a.abs()[:, :1] >= 2.0**-6
+        if a.shape == (126, 128):
+            rel = torch.where(normal & (b.abs()[:, :1] >= 2.0**-6).t(), err / mag, 0.0)
+            worst = max(worst, float(rel.max()))
+    assert worst < 2.0**-10
