@@ -299,6 +299,8 @@ def _norm_args(name, x, norm, residual):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x needs a last dimension of at least 1, got {tuple(x.shape)}")
     n = x.shape[-1]
+    if isinstance(norm, torch.nn.LayerNorm) or getattr(norm, "bias", None) is not None:
+        raise TypeError(f"{name}: {type(norm).__name__} is no root-mean-square norm")
     w, eps = norm.weight, norm.eps
     if w is None:
         if tuple(norm.normalized_shape) != (n,):

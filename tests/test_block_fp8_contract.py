@@ -546,3 +546,13 @@ def test_what_the_matrix_instruction_cuts(dev, kernel):
             rel = torch.where(normal & (b.abs()[:, :1] >= 2.0**-6).t(), err / mag, 0.0)
             worst = max(worst, float(rel.max()))
     assert worst < 2.0**-10
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_another_kind_of_norm_is_refused(dev):
+    """A layer norm has all that is read of an nn.RMSNorm, and means something else."""
+    x = torch.zeros(3, 16, device=dev)
+    for norm in (nn.LayerNorm(16), nn.LayerNorm(16, bias=False), nn.LayerNorm(16, elementwise_affine=False)):
+        for f in (Fx.rms_norm, Fx.rms_norm_fp8):
+            with pytest.raises(TypeError, match="LayerNorm"), torch.no_grad():
+                f(x, norm.to(dev))
