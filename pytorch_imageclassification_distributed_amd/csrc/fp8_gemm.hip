@@ -348,7 +348,7 @@ __global__ __launch_bounds__(512) void fp8_gemm_few_kernel(const Fp8Gemm p) {
 // 256 x 256 with the ring kernel's schedule, same size: 8 waves of 64 x 128 313 us, of 128 x 64 342, 4 of 128 x 128 482 (it
 // spills there: the builtin's accumulators and the fragments share the file), 128 x 128 tiles 405; this schedule needs the
 // registers that only a lone wave of a SIMD has.
-// 8192 x 8192 x 4096: 211 us (2.6 PFLOP/s), 186 of it the main loop; with loads that always hit L2, or a prefetch into
+// 8192 x 8192 x 4096: 211 to 226 us by operands and clock (2.4 to 2.6 PFLOP/s), 186 of 211 the main loop; with loads that always hit L2, or a prefetch into
 // L2, no faster; without any load 170 (the clock under full load), so the matrix pipe bounds it.  The rest is the
 // epilogue and a block's first loads; persistent blocks that issue the next tile's loads before the outputs were slower
 // (249 us: their registers spill).
@@ -604,14 +604,18 @@ thread_local int g_force = -1;  // tests and measurements: this thread's calls r
 
 // Which kernel: the one whose time this estimates lowest, in us, from what each measured on 256 CUs - a round of blocks
 // costs so much a k-step, plus its first loads and its outputs.  Measured (K 4096 unless given; kernel: us):
-//   16 x 4096        few16 7.0   64x64 10.2   128x64 -     128x128(4) -     128x128(2) 29   256 46
-//   32 x 4096        few32 9.7   64x64 10.2
-//   64 x 4096        few32 16.4  64x64 11.1
-//   512 x 4096                   64x64 22.8   128x64 19.0  128x128(4) 24.1  128x128(2) 32   256 42
-//   1024 x 4096                  64x64 42.2   128x64 35.1  128x128(4) 27.0  128x128(2) 35   256 42
-//   2048 x 4096                  64x64 82.6   128x64 73.6  128x128(4) 57.2  128x128(2) 50   256 58
-//   4096 x 4096                  64x64 161    128x64 147   128x128(4) 113   128x128(2) 101  256 65
-//   8192 x 2048, K 512           64x64 37.0   128x64 41.2  128x128(4) 33.1  128x128(2) 25   256 19
+//   16 x 4096        few16 7.5   64x64 9.9    128x64 12.6  128x128(4) 19.5  128x128(2) 25   256 38
+//   32 x 4096        few32 10.2  64x64 10.4
+//   64 x 4096        few32 17.3  64x64 11.3
+//   512 x 4096                   64x64 23.2   128x64 18.4  128x128(4) 23.9  128x128(2) 33   256 42
+//   1024 x 4096                  64x64 42.2   128x64 34.5  128x128(4) 27.5  128x128(2) 35   256 42
+//   2048 x 4096                  64x64 79.6   128x64 64.7  128x128(4) 52.4  128x128(2) 48   256 44
+//   4096 x 4096                  64x64 161    128x64 136   128x128(4) 107   128x128(2) 97   256 58
+//   8192 x 8192                  64x64 623    128x64 533   128x128(4) 432   128x128(2) 456  256 226
+//   8192 x 2048, K 512           64x64 31.8   128x64 36.5  128x128(4) 30.6  128x128(2) 24   256 18
+// The constants come from launches that leave part of the chip idle; under full load its clock is lower, and the estimate
+// 15 to 25 % short for the two widest tiles (8192 x 8192: 178 of 226; 4096 x 4096: 45 of 58).  That changes the choice
+// where they lie within that of each other: 2048 x 4096 takes 128x128(2), 7 % above the best.
 enum { K_FEW16, K_FEW32, K_64, K_128x64, K_128_4, K_128_2, K_256, K_COUNT };
 
 double estimate(int k, const Fp8Gemm& p) {
