@@ -13,7 +13,7 @@
 //    registers half 0 just released (two fragment sets in all, 96 VGPRs at 128 x 64 a wave);
 //  * 8 waves, two a SIMD: 128 x 64 a wave for 256 x 256 (2 x 4), 64 x 64 for 256 x 128 (4 x 2) and 512 x 64 (8 x 1), the
 //    accumulators (128 or 64 registers a lane) in AGPRs.  The split was taken by measurement with this schedule (grouped,
-//    spread variant; us of a bare GEMM M x N x K; one box, profiles/deep_conv_wave_layouts.txt):
+//    spread variant; us of a bare GEMM M x N x K; one GPU, profiles/deep_conv_wave_layouts.txt):
 //      256 x 256 on               4096^3   8192^3   50176x512x2048   50176x2048x512   200704x1024x256
 //      8 waves, 2 x 4               99.3    743.5             99.6            129.3             200.2
 //      8 waves, 4 x 2               99.0    739.6             99.6            129.7             200.6
@@ -21,9 +21,9 @@
 //      4 waves, 1 x 4              100.5    740.1            104.8            143.3             224.3
 //      4 waves, 4 x 1              100.9    737.8            104.9            148.7             229.9
 //      (one tile in flight, 2 x 4) 107.3    919.0            105.1            122.0             192.0
-//    Long sums do not tell the splits apart (the LDS port has room in all of them: a k-step reads 96 to 160 KB beside the
-//    64 KB that land, in the 2048 cycles of its MFMAs); with short ones the second wave of a SIMD hides the first loads
-//    and the outputs of the other;
+//    Long sums do not tell the splits apart: a k-step reads 128 KB (2 x 2) to 192 KB (8 waves) of LDS beside the 64 KB
+//    that land, 1536 to 2048 cycles of its port, its MFMAs take 2048, and the step about 3400 (8192^3).  With short ones
+//    the second wave of a SIMD hides the first loads and the outputs of the other;
 //  * the gather (LDS-DMA with per-lane im2col source offsets, zero padding = an out-of-range offset),
 //    the source-side XOR swizzle, the XCD-aware block remap and the fused epilogues are those of
 //    conv_gemm_glds_kernel (conv_common.h), so both kernels write identical tiles.
