@@ -7,7 +7,7 @@
 // the largest (the sum of the two operands' exponents; a subnormal counts with its format's least, -6); the groups' sums
 // keep float32's bits.  So an output is off by at most 7 x 2^-13 of the groups' largest such powers added up: 2^-10.2 of
 // sum |a||b| where the largest products are of normal values, more where they are not.  That takes one large product
-// beside seven just below the cut; measured are 2^-12.1 of sum |a||b| at most on random bytes (K 128; 2^-14.5 at 1024), and
+// beside seven just below the cut; measured are 2^-12.0 of sum |a||b| at most on random bytes (K 128; 2^-14.5 at 1024), and
 // 1.5e-5 of the result's norm on normal data, whatever K (the bf16 instruction: 9e-8).  Nothing bounds it relative to a
 // result whose terms cancel.
 #include <type_traits>

@@ -1,6 +1,8 @@
 """What the documentation of the pre-norm 8-bit linear block (ops/functional.py dropout_counter, rms_norm, rms_norm_fp8,
 quantize_fp8, matmul_fp8, linear_fp8) allows or refuses beyond plain calls: forward-mode tangents, operands that a user
 lays out, unusual sizes, calls from several threads."""
+import contextlib
+
 import pytest
 import torch
 import torch.nn as nn
@@ -532,7 +534,6 @@ def test_what_the_matrix_instruction_cuts(dev, kernel):
         qb = plain_blocks(b, dev)
         if kernel == 6:  # (the large tile takes 128 x 128 scales: the same, all 1)
             qb = fb.Fp8Blocks(qb.q, qb.scale[:1].contiguous(), qb.shape, 128)
-        import contextlib
         with (forced(kernel) if dev == "cuda" else contextlib.nullcontext()):
             y = Fx.matmul_fp8(qa, qb, out_dtype=torch.float32).double().cpu()
         err = (y - a.double() @ b.double().t()).abs()
